@@ -69,6 +69,57 @@ type Shape struct {
 	Bias  float64
 }
 
+// Element types, activations and limits of the channels-last operators
+// (include/simtgo_b200.h).
+const (
+	TypeF32               int32 = 0
+	TypeBF16              int32 = 1
+	TypeF16               int32 = 2
+	ActNone               int32 = 0
+	ActSiLU               int32 = 1
+	ActGELU               int32 = 2
+	ActSoftclip           int32 = 3
+	GroupNormMaxChannels        = 8192
+	GroupNormMaxPositions       = 1 << 30
+)
+
+// GroupNormConfig mirrors simtgo_group_norm: pitches in elements, x the
+// input, y the output or its gradient, d the input's gradient.
+type GroupNormConfig struct {
+	XSample   int64
+	XRow      int64
+	YSample   int64
+	YRow      int64
+	DSample   int64
+	DRow      int64
+	Samples   int32
+	Positions int32
+	Channels  int32
+	Groups    int32
+	Type      int32
+	ParamType int32
+	Act       int32
+	Block     int32
+	ActParam  float32
+	Eps       float32
+}
+
+// GatedUnitConfig mirrors simtgo_gated_unit.
+type GatedUnitConfig struct {
+	Rows     int64
+	APitch   int64
+	BPitch   int64
+	YPitch   int64
+	DAPitch  int64
+	DBPitch  int64
+	Channels int32
+	Type     int32
+	Act      int32
+	Block    int32
+	ActParam float32
+	Reserved int32
+}
+
 // The library's entry points, one variable per function of
 // include/simtgo_b200.h, bound by Load.
 var (
@@ -111,6 +162,15 @@ var (
 	HistogramAllreduce              func(comm uintptr, bins uintptr, binsLen int32, x uintptr, xLen int64, stream uintptr) int32
 	HistogramAllreduceFused         func(comm uintptr, bins uintptr, binsLen int32, x uintptr, xLen int64, stream uintptr) int32
 	HistogramAllreduceFusedOverwrite func(comm uintptr, bins uintptr, binsLen int32, x uintptr, xLen int64, stream uintptr) int32
+
+	// The channels-last operators: group norm with an activation, 8-bit
+	// checkpoints and the gated unit (0 for a buffer that is not passed).
+	GroupNorm         func(y uintptr, mean uintptr, rstd uintptr, x uintptr, weight uintptr, bias uintptr, lengths uintptr, codes uintptr, scales uintptr, cfg *GroupNormConfig, stream uintptr) int32
+	GroupNormBackward func(dx uintptr, dweight uintptr, dbias uintptr, dy uintptr, x uintptr, codes uintptr, scales uintptr, mean uintptr, rstd uintptr, weight uintptr, bias uintptr, lengths uintptr, cfg *GroupNormConfig, stream uintptr) int32
+	Pack8             func(codes uintptr, scales uintptr, x uintptr, elemType int32, rows int64, channels int32, rowPitch int64, block int32, stream uintptr) int32
+	Unpack8           func(x uintptr, codes uintptr, scales uintptr, elemType int32, rows int64, channels int32, rowPitch int64, block int32, stream uintptr) int32
+	Gated             func(y uintptr, a uintptr, b uintptr, aCodes uintptr, aScales uintptr, bCodes uintptr, bScales uintptr, cfg *GatedUnitConfig, stream uintptr) int32
+	GatedBackward     func(da uintptr, db uintptr, dy uintptr, a uintptr, b uintptr, aCodes uintptr, aScales uintptr, bCodes uintptr, bScales uintptr, cfg *GatedUnitConfig, stream uintptr) int32
 
 	// The tile track (package tile): a graph handle is a uintptr, a tensor
 	// its node id (int32, -1 on a latched error).
@@ -201,6 +261,13 @@ func bind(h uintptr) {
 	purego.RegisterLibFunc(&HistogramAllreduce, h, "simtgo_Histogram_allreduce")
 	purego.RegisterLibFunc(&HistogramAllreduceFused, h, "simtgo_Histogram_allreduce_fused")
 	purego.RegisterLibFunc(&HistogramAllreduceFusedOverwrite, h, "simtgo_Histogram_allreduce_fused_overwrite")
+
+	purego.RegisterLibFunc(&GroupNorm, h, "simtgo_GroupNorm")
+	purego.RegisterLibFunc(&GroupNormBackward, h, "simtgo_GroupNorm_backward")
+	purego.RegisterLibFunc(&Pack8, h, "simtgo_Pack8")
+	purego.RegisterLibFunc(&Unpack8, h, "simtgo_Unpack8")
+	purego.RegisterLibFunc(&Gated, h, "simtgo_Gated")
+	purego.RegisterLibFunc(&GatedBackward, h, "simtgo_Gated_backward")
 
 	purego.RegisterLibFunc(&TileNew, h, "simtgo_tile_new")
 	purego.RegisterLibFunc(&TileFree, h, "simtgo_tile_free")

@@ -259,6 +259,109 @@ int simtgo_Histogram_allreduce_fused_overwrite(simtgo_comm* comm, int32_t* bins,
                                                int32_t bins_len, const int32_t* x, int64_t x_len,
                                                void* stream);
 
+/* ---- channels-last operators (no counterpart in the reference) ----------
+ * Normalisation, gating and 8-bit checkpoints of batches of channels-last
+ * samples (interleaved signals and images), forward and backward: what a
+ * training step runs beside Softclip and Quantize. A batch is `samples` samples
+ * of `positions` rows of `channels` consecutive elements; row s of sample n
+ * starts n*sample_pitch + s*row_pitch elements into its buffer (both pitches
+ * free, so slices, crops and time-major batches need no copy). Extents are
+ * 64-bit. Every buffer is device memory, aligned to its element type; rows on
+ * 16-byte boundaries are fastest. Arithmetic is float32 with one rounding to
+ * the element type at the end; sums run in a fixed order, so equal inputs give
+ * equal bits. Written buffers must not overlap any other buffer of the call,
+ * nor a row another row of the same buffer (SIMTGO_EALIAS). Configurations are
+ * HOST pointers, read before the call returns. */
+
+/* Element types. */
+enum { SIMTGO_F32 = 0, SIMTGO_BF16 = 1, SIMTGO_F16 = 2 };
+
+/* Activations: z; z/(1+exp(-z)); z*Phi(z) with the normal distribution
+ * function Phi; Softclip's curve (kernels/softclip.go:11-23) with threshold
+ * act_param >= 0. */
+enum {
+    SIMTGO_ACT_NONE = 0,
+    SIMTGO_ACT_SILU = 1,
+    SIMTGO_ACT_GELU = 2,
+    SIMTGO_ACT_SOFTCLIP = 3
+};
+
+/* Most channels of a group-normalised batch, and most positions of a sample. */
+#define SIMTGO_GROUP_NORM_MAX_CHANNELS 8192
+#define SIMTGO_GROUP_NORM_MAX_POSITIONS (1 << 30)
+
+/* Pitches are in elements. x: the input; y: the forward output, or in the
+ * backward pass its gradient dy; d: the backward output dx. Unused ones are
+ * ignored. block: channels per checkpoint scale (32, 64, 128 or 256), read
+ * only when a checkpoint is passed. */
+typedef struct simtgo_group_norm {
+    int64_t x_sample, x_row, y_sample, y_row, d_sample, d_row;
+    int32_t samples, positions, channels, groups;
+    int32_t type, param_type, act, block;
+    float act_param, eps;
+} simtgo_group_norm;
+
+/* Group norm with an activation. Group g of a sample holds channels
+ * [g*D, (g+1)*D), D = channels/groups, of its valid positions: all of them, or
+ * the first lengths[n] of sample n (device int32, clamped to [0, positions];
+ * NULL: all). mean and rstd = 1/sqrt(var + eps) are float32, samples*groups,
+ * and either may be NULL; y = act((x - mean)*rstd*weight + bias). weight and
+ * bias are `channels` elements of param_type (NULL: ones, zeros). Positions past
+ * a sample's length are neither read nor written, in any buffer; an empty
+ * sample has mean 0 and rstd 1/sqrt(eps). eps is positive. With codes (and
+ * scales) the 8-bit checkpoint of x is written in the same pass: what
+ * simtgo_Pack8 writes for the samples*positions rows of x. */
+int simtgo_GroupNorm(void* y, float* mean, float* rstd, const void* x, const void* weight,
+                     const void* bias, const int32_t* lengths, int8_t* codes, float* scales,
+                     const simtgo_group_norm* cfg, void* stream);
+
+/* The gradients of simtgo_GroupNorm, from its mean and rstd and either x or
+ * the checkpoint it wrote (exactly one of x and codes is given). With
+ * xh = (x - mean)*rstd, z = xh*weight + bias and dz = dy*act'(z):
+ * dweight = sum dz*xh and dbias = sum dz over all samples and valid positions
+ * (float32, overwritten), and dx = rstd*(dz*weight - s1 - xh*s2) with s1, s2
+ * the group's means of dz*weight and dz*weight*xh. dx, dweight and dbias may
+ * each be NULL. */
+int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void* dy,
+                              const void* x, const int8_t* codes, const float* scales,
+                              const float* mean, const float* rstd, const void* weight,
+                              const void* bias, const int32_t* lengths,
+                              const simtgo_group_norm* cfg, void* stream);
+
+/* An 8-bit checkpoint of a matrix of `rows` rows, row_pitch elements apart.
+ * Each block of `block` consecutive channels of a row (the last one may be
+ * shorter) has a = max(largest magnitude, 2^-100), scale = a/127 and codes
+ * rint(x * (127/a)), every step rounded to float32, ties to even. A block with
+ * a NaN or an infinity gets scale NaN. codes is rows*channels bytes, scales
+ * rows*ceil(channels/block) floats, both contiguous. */
+int simtgo_Pack8(int8_t* codes, float* scales, const void* x, int32_t type, int64_t rows,
+                 int32_t channels, int64_t row_pitch, int32_t block, void* stream);
+/* x = code * scale, rounded to the type. */
+int simtgo_Unpack8(void* x, const int8_t* codes, const float* scales, int32_t type, int64_t rows,
+                   int32_t channels, int64_t row_pitch, int32_t block, void* stream);
+
+/* a, b: the two inputs; y: the forward output, or its gradient dy; da, db: the
+ * backward outputs. Pitches in elements; unused ones are ignored. block: as
+ * above, read only when a checkpoint is passed. */
+typedef struct simtgo_gated_unit {
+    int64_t rows, a_pitch, b_pitch, y_pitch, da_pitch, db_pitch;
+    int32_t channels, type, act, block;
+    float act_param;
+    int32_t reserved;
+} simtgo_gated_unit;
+
+/* y = act(a)*b, or act(a) where b is NULL. With a_codes and a_scales the
+ * checkpoint of a, with b_codes and b_scales that of b, is written in the same
+ * pass (what simtgo_Pack8 writes). */
+int simtgo_Gated(void* y, const void* a, const void* b, int8_t* a_codes, float* a_scales,
+                 int8_t* b_codes, float* b_scales, const simtgo_gated_unit* cfg, void* stream);
+/* da = dy*b*act'(a) and db = dy*act(a), from a and b or from their checkpoints
+ * (a or a_codes; for a gated unit b or b_codes, of the same kind as a's). da
+ * and db may each be NULL; without b there is no db. */
+int simtgo_Gated_backward(void* da, void* db, const void* dy, const void* a, const void* b,
+                          const int8_t* a_codes, const float* a_scales, const int8_t* b_codes,
+                          const float* b_scales, const simtgo_gated_unit* cfg, void* stream);
+
 /* ---- the tile track (package tile) -------------------------------------- */
 
 /* tile/tile.go:22 BlockSize and :25 MaxTaps. */

@@ -34,6 +34,23 @@ class Shape(C.Structure):
     _fields_ = [("floor_gain", C.c_float), ("count", C.c_int32), ("bias", C.c_double)]
 
 
+class GroupNormConfig(C.Structure):
+    """simtgo_group_norm: the extents, pitches and options of a group norm."""
+    _fields_ = [(n, C.c_int64) for n in ("x_sample", "x_row", "y_sample", "y_row", "d_sample",
+                                         "d_row")] + \
+               [(n, C.c_int32) for n in ("samples", "positions", "channels", "groups", "type",
+                                         "param_type", "act", "block")] + \
+               [("act_param", C.c_float), ("eps", C.c_float)]
+
+
+class GatedUnitConfig(C.Structure):
+    """simtgo_gated_unit: the extents, pitches and options of a gated unit."""
+    _fields_ = [(n, C.c_int64) for n in ("rows", "a_pitch", "b_pitch", "y_pitch", "da_pitch",
+                                         "db_pitch")] + \
+               [(n, C.c_int32) for n in ("channels", "type", "act", "block")] + \
+               [("act_param", C.c_float), ("reserved", C.c_int32)]
+
+
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 _SIGS = {
     "simtgo_last_error": [],
@@ -66,6 +83,12 @@ _SIGS = {
     "simtgo_Histogram_allreduce": [_vp, _vp, _i32, _vp, _i64, _vp],
     "simtgo_Histogram_allreduce_fused": [_vp, _vp, _i32, _vp, _i64, _vp],
     "simtgo_Histogram_allreduce_fused_overwrite": [_vp, _vp, _i32, _vp, _i64, _vp],
+    "simtgo_GroupNorm": [_vp] * 9 + [_vp, _vp],
+    "simtgo_GroupNorm_backward": [_vp] * 12 + [_vp, _vp],
+    "simtgo_Pack8": [_vp, _vp, _vp, _i32, _i64, _i32, _i64, _i32, _vp],
+    "simtgo_Unpack8": [_vp, _vp, _vp, _i32, _i64, _i32, _i64, _i32, _vp],
+    "simtgo_Gated": [_vp] * 7 + [_vp, _vp],
+    "simtgo_Gated_backward": [_vp] * 9 + [_vp, _vp],
     "simtgo_tile_new": [],
     "simtgo_tile_free": [_vp],
     "simtgo_tile_input": [_vp, _vp, _i32],

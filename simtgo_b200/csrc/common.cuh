@@ -50,6 +50,11 @@ int watchdog_check_and_clear(uint32_t* bits);
 // Private resources released by simtgo_shutdown (fir.cu).
 int fir_host_release();
 int tile_pool_release();  // trims the tile reductions' scratch pools (simtgo_shutdown)
+// Stream-ordered scratch of the current device from the library's own pool
+// (tile.cu); the caller frees it with cudaFreeAsync on the same stream. Under
+// stream capture it becomes an allocation of the graph itself, so captured
+// graphs share none.
+int scratch_alloc(void** p, size_t bytes, cudaStream_t s);
 int tile_jit_release();   // unloads the specialised tile kernels' modules (simtgo_shutdown)
 
 // ---- launch-contract checks (simt/kernel.go:293-369, :488-514) -------------

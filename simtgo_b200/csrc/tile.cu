@@ -884,6 +884,13 @@ int scratch_pool(cudaMemPool_t* out) {
 }  // namespace
 
 namespace sg {
+int scratch_alloc(void** p, size_t bytes, cudaStream_t s) {
+    cudaMemPool_t pool;
+    if (int rc = scratch_pool(&pool)) return rc;
+    return cuda_status(cudaMallocFromPoolAsync(p, std::max<size_t>(bytes, 16), pool, s),
+                       "cudaMallocFromPoolAsync");
+}
+
 int tile_pool_release() {
     std::lock_guard<std::mutex> lk(g_pool_mu);
     for (int dev = 0; dev < 64; dev++)
@@ -905,10 +912,7 @@ struct AsyncBuf {
     }
     int alloc(size_t bytes, cudaStream_t st) {
         s = st;
-        cudaMemPool_t pool;
-        if (int rc = scratch_pool(&pool)) return rc;
-        return sg::cuda_status(cudaMallocFromPoolAsync(&p, std::max<size_t>(bytes, 16), pool, st),
-                               "cudaMallocFromPoolAsync");
+        return sg::scratch_alloc(&p, bytes, st);
     }
 };
 
