@@ -119,54 +119,69 @@ __device__ __forceinline__ void st_unit(T* p, const Raw<T>& r, int cnt) {
     }
 }
 
-__device__ __forceinline__ void unpack(const Raw<float>& r, float (&v)[8]) {
+// Eight values as four pairs: Blackwell's packed float32 instructions take two
+// at once, each rounded as the scalar ones are, which halves the instructions
+// of kernels that issue slots would otherwise bound before HBM does.
+struct V8 {
+    float2 p[4];
+};
+
+// The assembler may contract a packed product with the addition after it: where
+// the product's own rounding counts (the checkpoint's codes) it is scalar.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 neg2(float2 v) { return make_float2(-v.x, -v.y); }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return add2(a, neg2(b)); }
+
+__device__ __forceinline__ V8 unpack(const Raw<float>& r) {
+    V8 v;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        v[4 * i] = __uint_as_float(r.q[i].x);
-        v[4 * i + 1] = __uint_as_float(r.q[i].y);
-        v[4 * i + 2] = __uint_as_float(r.q[i].z);
-        v[4 * i + 3] = __uint_as_float(r.q[i].w);
+        v.p[2 * i] = make_float2(__uint_as_float(r.q[i].x), __uint_as_float(r.q[i].y));
+        v.p[2 * i + 1] = make_float2(__uint_as_float(r.q[i].z), __uint_as_float(r.q[i].w));
     }
+    return v;
 }
-__device__ __forceinline__ void unpack(const Raw<__nv_bfloat16>& r, float (&v)[8]) {
+__device__ __forceinline__ V8 unpack(const Raw<__nv_bfloat16>& r) {
     const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
+    V8 v;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; i++)
+        v.p[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    return v;
 }
-__device__ __forceinline__ void unpack(const Raw<__half>& r, float (&v)[8]) {
+__device__ __forceinline__ V8 unpack(const Raw<__half>& r) {
     const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
+    V8 v;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
+    for (int i = 0; i < 4; i++) v.p[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    return v;
 }
 
 // Rounded to nearest even, once.
-__device__ __forceinline__ void pack(const float (&v)[8], Raw<float>& r) {
+__device__ __forceinline__ void pack(const V8& v, Raw<float>& r) {
 #pragma unroll
     for (int i = 0; i < 2; i++)
-        r.q[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
-                            __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+        r.q[i] = make_uint4(__float_as_uint(v.p[2 * i].x), __float_as_uint(v.p[2 * i].y),
+                            __float_as_uint(v.p[2 * i + 1].x), __float_as_uint(v.p[2 * i + 1].y));
 }
-__device__ __forceinline__ void pack(const float (&v)[8], Raw<__nv_bfloat16>& r) {
+__device__ __forceinline__ void pack(const V8& v, Raw<__nv_bfloat16>& r) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        const __nv_bfloat162 h = __float22bfloat162_rn(v.p[i]);
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     r.q[0] = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void pack(const float (&v)[8], Raw<__half>& r) {
+__device__ __forceinline__ void pack(const V8& v, Raw<__half>& r) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        const __half2 h = __float22half2_rn(v.p[i]);
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     r.q[0] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -181,96 +196,152 @@ __device__ __forceinline__ float ld_param(const void* p, int type, int64_t i) {
 }
 
 // ---- activations --------------------------------------------------------------
-// Two-byte types take the special-function unit's exponential and reciprocal
-// (a few 2^-22, far below their 2^-9 and 2^-12 half steps): the exact ones
-// would bind the kernels before HBM does. float32 keeps expf, erff and IEEE
+// Two-byte types take the special-function unit's exp2 and reciprocal (a few
+// 2^-22, far below their 2^-9 and 2^-12 half steps): the exact functions would
+// bind the kernels before HBM does. float32 keeps expf, erfcf and IEEE
 // division.
 
+__device__ __forceinline__ float ex2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// For 1 <= x, where a flushed result is one that no sum notices.
+__device__ __forceinline__ float rcp_ftz(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 __device__ __forceinline__ float rcp_fast(float x) {
     float r;
     asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-
-template <bool kFast>
-__device__ __forceinline__ float sigmoid(float z) {
-    return kFast ? __fdividef(1.0f, 1.0f + __expf(-z)) : __fdiv_rn(1.0f, 1.0f + expf(-z));
+// min and max that keep a NaN.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-// Phi(z), the normal distribution function, and e = exp(-z^2/2). The fast
-// form is Abramowitz and Stegun's 7.1.26 for erf (Hastings), within 1.5e-7,
-// in the variable t = 1/(1 + p |z|/sqrt 2); the negative side is taken from
-// the complement itself, so it does not cancel.
 template <bool kFast>
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
-    if (!kFast) {
-        e = expf(-0.5f * z * z);
-        return 0.5f * erfcf(-0.70710678f * z);
-    }
-    const float x = fabsf(z) * 0.70710678f;
-    const float t = __fdividef(1.0f, __fmaf_rn(0.3275911f, x, 1.0f));
-    e = __expf(-x * x);
-    float q = __fmaf_rn(1.061405429f, t, -1.453152027f);
-    q = __fmaf_rn(q, t, 1.421413741f);
-    q = __fmaf_rn(q, t, -0.284496736f);
-    q = __fmaf_rn(q, t, 0.254829592f);
-    q = 0.5f * q * t * e;  // Phi(-|z|)
-    return z < 0.0f ? q : 1.0f - q;
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+    if (!kFast)
+        return make_float2(__fdiv_rn(1.0f, 1.0f + expf(-z.x)), __fdiv_rn(1.0f, 1.0f + expf(-z.y)));
+    const float2 e = mul2(z, both(-1.44269504f));
+    const float2 d = add2(make_float2(ex2_fast(e.x), ex2_fast(e.y)), both(1.0f));
+    return make_float2(rcp_ftz(d.x), rcp_ftz(d.y));
 }
 
-// softclip of kernels/softclip.go:11-23 and its slope factor 1/(1+over).
+// Fast GELU: with q = Phi(-|z|) and e = exp(-z^2/2), z*Phi(z) is
+// max(z, 0) - |z|*q. q is Abramowitz and Stegun's 7.1.26 for the complement of
+// erf (Hastings), within 0.75e-7, in t = 1/(1 + p |z|/sqrt 2); past |z| = 20 it
+// is zero in float32, so |z| stops there and no infinity meets a zero.
+struct Normal2 {
+    float2 az, q, e;
+};
+__device__ __forceinline__ Normal2 normal2(float2 z) {
+    Normal2 r;
+    r.az = make_float2(min_nan(fabsf(z.x), 20.0f), min_nan(fabsf(z.y), 20.0f));
+    const float2 d = fma2(r.az, both(0.3275911f * 0.70710678f), both(1.0f));
+    const float2 t = make_float2(rcp_ftz(d.x), rcp_ftz(d.y));
+    const float2 h = mul2(mul2(r.az, r.az), both(-0.5f * 1.44269504f));
+    r.e = make_float2(ex2_fast(h.x), ex2_fast(h.y));
+    // Half of the polynomial: the coefficients are halved.
+    float2 q = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
+    q = fma2(q, t, both(0.5f * 1.421413741f));
+    q = fma2(q, t, both(0.5f * -0.284496736f));
+    q = fma2(q, t, both(0.5f * 0.254829592f));
+    r.q = mul2(mul2(q, t), r.e);
+    return r;
+}
+__device__ __forceinline__ float2 gelu2(float2 z, const Normal2& n) {
+    return sub2(make_float2(max_nan(z.x, 0.0f), max_nan(z.y, 0.0f)), mul2(n.az, n.q));
+}
+
+// softclip of kernels/softclip.go:11-23 and its slope, 1 or 1/(1+over)^2.
 template <bool kFast>
 __device__ __forceinline__ float softclip(float z, float t, float& slope) {
     const float a = fabsf(z), over = a - t;
     const float r = kFast ? rcp_fast(1.0f + over) : __fdiv_rn(1.0f, 1.0f + over);
     const float shaped = t + (kFast ? over * r : __fdiv_rn(over, 1.0f + over));
     slope = a <= t ? 1.0f : r * r;
-    return a <= t ? z : z < 0.0f ? -shaped : shaped;
+    return a <= t ? z : copysignf(shaped, z);
 }
 
 // v <- act(v), eight at a time (one uniform branch per unit).
 template <bool kFast>
-__device__ __forceinline__ void activate(float (&v)[8], int act, float param) {
-    float s;
+__device__ __forceinline__ void activate(V8& v, int act, float param) {
     if (act == SIMTGO_ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= sigmoid<kFast>(v[i]);
+        for (int i = 0; i < 4; i++) v.p[i] = mul2(v.p[i], sigmoid2<kFast>(v.p[i]));
     } else if (act == SIMTGO_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= normal_cdf<kFast>(v[i], s);
+        for (int i = 0; i < 4; i++) {
+            if (kFast) {
+                v.p[i] = gelu2(v.p[i], normal2(v.p[i]));
+            } else {
+                v.p[i].x *= 0.5f * erfcf(-0.70710678f * v.p[i].x);
+                v.p[i].y *= 0.5f * erfcf(-0.70710678f * v.p[i].y);
+            }
+        }
     } else if (act == SIMTGO_ACT_SOFTCLIP) {
+        float s;
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = softclip<kFast>(v[i], param, s);
+        for (int i = 0; i < 4; i++) {
+            v.p[i].x = softclip<kFast>(v.p[i].x, param, s);
+            v.p[i].y = softclip<kFast>(v.p[i].y, param, s);
+        }
     }
 }
 
 // f <- act(z), d <- act'(z).
 template <bool kFast>
-__device__ __forceinline__ void activate_slope(const float (&z)[8], float (&f)[8], float (&d)[8],
-                                               int act, float param) {
+__device__ __forceinline__ void activate_slope(const V8& z, V8& f, V8& d, int act, float param) {
     if (act == SIMTGO_ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float s = sigmoid<kFast>(z[i]);
-            f[i] = z[i] * s;
-            d[i] = __fmaf_rn(f[i], 1.0f - s, s);
+        for (int i = 0; i < 4; i++) {
+            const float2 s = sigmoid2<kFast>(z.p[i]);
+            f.p[i] = mul2(z.p[i], s);
+            d.p[i] = fma2(f.p[i], sub2(both(1.0f), s), s);
         }
     } else if (act == SIMTGO_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            float e;
-            const float p = normal_cdf<kFast>(z[i], e);
-            f[i] = z[i] * p;
-            d[i] = __fmaf_rn(z[i] * 0.39894228f, e, p);
+        for (int i = 0; i < 4; i++) {
+            if (kFast) {
+                const Normal2 n = normal2(z.p[i]);
+                f.p[i] = gelu2(z.p[i], n);
+                // Phi = 1/2 +- (1/2 - q), and z*phi with |z| stopped as above.
+                const float2 h = sub2(both(0.5f), n.q);
+                const float2 c = add2(
+                    both(0.5f), make_float2(copysignf(h.x, z.p[i].x), copysignf(h.y, z.p[i].y)));
+                const float2 zc =
+                    make_float2(copysignf(n.az.x, z.p[i].x), copysignf(n.az.y, z.p[i].y));
+                d.p[i] = fma2(mul2(zc, both(0.39894228f)), n.e, c);
+            } else {
+                const float px = 0.5f * erfcf(-0.70710678f * z.p[i].x);
+                const float py = 0.5f * erfcf(-0.70710678f * z.p[i].y);
+                f.p[i] = make_float2(z.p[i].x * px, z.p[i].y * py);
+                d.p[i].x = __fmaf_rn(z.p[i].x * 0.39894228f, expf(-0.5f * z.p[i].x * z.p[i].x), px);
+                d.p[i].y = __fmaf_rn(z.p[i].y * 0.39894228f, expf(-0.5f * z.p[i].y * z.p[i].y), py);
+            }
         }
     } else if (act == SIMTGO_ACT_SOFTCLIP) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = softclip<kFast>(z[i], param, d[i]);
+        for (int i = 0; i < 4; i++) {
+            f.p[i].x = softclip<kFast>(z.p[i].x, param, d.p[i].x);
+            f.p[i].y = softclip<kFast>(z.p[i].y, param, d.p[i].y);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            f[i] = z[i];
-            d[i] = 1.0f;
+        for (int i = 0; i < 4; i++) {
+            f.p[i] = z.p[i];
+            d.p[i] = both(1.0f);
         }
     }
 }
@@ -287,14 +358,72 @@ struct Codes {
     uint2 q;  // eight signed bytes
 };
 
-__device__ __forceinline__ uint32_t largest(const float (&v)[8]) {
-    uint32_t m = 0;
+// Bit patterns of the largest magnitudes of the blocks that U rows' units lie
+// in, over the `lanes` (a power of two) neighbouring lanes that hold a block.
+// Every lane of the warp calls it. Two-byte types carry two rows in a
+// register's halves.
+template <int U>
+__device__ __forceinline__ void block_max(const Raw<float> (&raw)[U], int lanes,
+                                          uint32_t (&m)[U]) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-    return m;
+    for (int u = 0; u < U; u++) {
+        m[u] = 0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint4 q = raw[u].q[i];
+            m[u] = max(max(m[u], max(q.x & 0x7fffffffu, q.y & 0x7fffffffu)),
+                       max(q.z & 0x7fffffffu, q.w & 0x7fffffffu));
+        }
+    }
+    for (int off = lanes / 2; off; off /= 2)
+#pragma unroll
+        for (int u = 0; u < U; u++) m[u] = max(m[u], __shfl_xor_sync(~0u, m[u], off));
+}
+template <int U>
+__device__ __forceinline__ void block_max16(const uint4 (&raw)[U], int lanes, uint32_t (&m)[U]) {
+    static_assert(U % 2 == 0, "rows go in pairs");
+    uint32_t pair[U / 2];
+#pragma unroll
+    for (int u = 0; u < U; u += 2) {
+        uint32_t h[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint4 q = raw[u + j];
+            h[j] = __vmaxu2(__vmaxu2(q.x & 0x7fff7fffu, q.y & 0x7fff7fffu),
+                            __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu));
+        }
+        pair[u / 2] = __vmaxu2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[0], h[1], 0x7632));
+    }
+    for (int off = lanes / 2; off; off /= 2)
+#pragma unroll
+        for (int u = 0; u < U / 2; u++)
+            pair[u] = __vmaxu2(pair[u], __shfl_xor_sync(~0u, pair[u], off));
+#pragma unroll
+    for (int u = 0; u < U; u++) m[u] = u & 1 ? pair[u / 2] >> 16 : pair[u / 2] & 0xffffu;
+}
+template <int U>
+__device__ __forceinline__ void block_max(const Raw<__nv_bfloat16> (&raw)[U], int lanes,
+                                          uint32_t (&m)[U]) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) q[u] = raw[u].q[0];
+    block_max16<U>(q, lanes, m);
+#pragma unroll
+    for (int u = 0; u < U; u++) m[u] <<= 16;
+}
+template <int U>
+__device__ __forceinline__ void block_max(const Raw<__half> (&raw)[U], int lanes,
+                                          uint32_t (&m)[U]) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) q[u] = raw[u].q[0];
+    block_max16<U>(q, lanes, m);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        m[u] = __float_as_uint(__half2float(__ushort_as_half((unsigned short)m[u])));
 }
 
-// The block's scale and its inverse from the bit pattern of its largest
+// A block's scale and its inverse from the bit pattern of its largest
 // magnitude.
 __device__ __forceinline__ void block_scale(uint32_t m, float& scale, float& inverse) {
     if (m >= 0x7f800000u) {
@@ -310,11 +439,16 @@ __device__ __forceinline__ void block_scale(uint32_t m, float& scale, float& inv
 // rint(v * inverse) as signed bytes: adding 1.5 * 2^23 leaves the rounded
 // whole number (nearest even) in the low mantissa bits, whose low byte is its
 // two's complement.
-__device__ __forceinline__ Codes encode(const float (&v)[8], float inverse) {
+__device__ __forceinline__ Codes encode(const V8& v, float inverse) {
     uint32_t b[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        b[i] = __float_as_uint(__fadd_rn(__fmul_rn(v[i], inverse), 12582912.0f));
+    for (int i = 0; i < 4; i++) {
+        const float2 q =
+            make_float2(__fmul_rn(v.p[i].x, inverse), __fmul_rn(v.p[i].y, inverse));
+        const float2 r = add2(q, both(12582912.0f));
+        b[2 * i] = __float_as_uint(r.x);
+        b[2 * i + 1] = __float_as_uint(r.y);
+    }
     Codes c;
     c.q.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     c.q.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
@@ -324,13 +458,18 @@ __device__ __forceinline__ Codes encode(const float (&v)[8], float inverse) {
 // What the codes stand for, in float32: fl(code * scale). A byte k with its
 // sign bit flipped is k + 128; placed under the exponent of 2^23 it reads as
 // 2^23 + 128 + k, exactly.
-__device__ __forceinline__ void decode(const Codes& c, float scale, float (&v)[8]) {
+__device__ __forceinline__ V8 decode(const Codes& c, float scale) {
     const uint32_t w[2] = {c.q.x ^ 0x80808080u, c.q.y ^ 0x80808080u};
+    V8 v;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t u = __byte_perm(w[i / 4], 0x4b000000u, 0x7440 | (i & 3));
-        v[i] = __fmul_rn(__uint_as_float(u) - 8388736.0f, scale);
+    for (int i = 0; i < 4; i++) {
+        const uint32_t a = __byte_perm(w[i / 2], 0x4b000000u, 0x7440 | (2 * i & 3));
+        const uint32_t b = __byte_perm(w[i / 2], 0x4b000000u, 0x7440 | ((2 * i + 1) & 3));
+        v.p[i] = mul2(
+            add2(make_float2(__uint_as_float(a), __uint_as_float(b)), both(-8388736.0f)),
+            both(scale));
     }
+    return v;
 }
 
 template <bool kVec>
@@ -361,11 +500,57 @@ __device__ __forceinline__ void st_codes(int8_t* p, const Codes& c, int cnt) {
         if (i < cnt) p[i] = (int8_t)(w[i / 4] >> (8 * (i & 3)));
 }
 
-// Largest bit pattern over the `lanes` (a power of two) neighbouring lanes
-// that hold one block. Every lane of the warp calls it.
-__device__ __forceinline__ uint32_t block_max(uint32_t m, int lanes) {
-    for (int off = lanes / 2; off; off /= 2) m = max(m, __shfl_xor_sync(~0u, m, off));
-    return m;
+// Where a tensor's checkpoint lies, and how a row's units map to its blocks.
+struct Kept {
+    int8_t* codes;
+    float* scales;
+    int channels, nblk;  // bytes of codes and scales per row
+    int shift, lanes;    // log2(units per block); lanes that hold one block
+};
+
+// Writes the checkpoint of the units that a warp's lanes hold of U rows: unit
+// `unit` (cnt channels; only where unit_on) of rows row + u*step, where live[u].
+// Every lane of the warp calls it, with zeros where it has no unit; live is the
+// same for the lanes of a block. The two divisions of a block's scale are shared
+// out: lane u of each block's lanes makes row u's, where there are that many.
+template <class T, int AW, int U>
+__device__ __forceinline__ void keep_units(const Raw<T> (&raw)[U], const Kept& k, int64_t row,
+                                           int64_t step, const bool (&live)[U], int unit, int cnt,
+                                           bool unit_on) {
+    uint32_t m[U];
+    block_max<U>(raw, k.lanes, m);
+    float inverse[U];
+    const int blk = unit >> k.shift;
+    if (k.lanes >= U) {
+        const int mine = threadIdx.x & (U - 1);
+        uint32_t sel = m[0];
+        bool sel_on = live[0];
+#pragma unroll
+        for (int u = 1; u < U; u++) {
+            sel = mine == u ? m[u] : sel;
+            sel_on = mine == u ? live[u] : sel_on;
+        }
+        float scale, inv;
+        block_scale(sel, scale, inv);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            inverse[u] = __shfl_sync(~0u, inv, (threadIdx.x & 31 & ~(U - 1)) + u);
+        if (sel_on && unit % k.lanes == mine && blk < k.nblk)
+            k.scales[(row + mine * step) * k.nblk + blk] = scale;
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float scale;
+            block_scale(m[u], scale, inverse[u]);
+            if (live[u] && unit % k.lanes == 0 && blk < k.nblk)
+                k.scales[(row + u * step) * k.nblk + blk] = scale;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (unit_on && live[u])
+            st_codes<AW == 16>(k.codes + (row + u * step) * k.channels + unit * kUnit,
+                               encode(unpack(raw[u]), inverse[u]), cnt);
 }
 
 // ---- host helpers -------------------------------------------------------------------

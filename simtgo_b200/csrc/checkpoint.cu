@@ -107,6 +107,9 @@ RowGrid row_grid(int64_t rows, int channels, int block, int sms) {
     while (sg::ceil_div(rows, (int64_t)g.phases * g.iters) * g.tiles > 0x7fffffff) g.iters *= 2;
     return g;
 }
+Kept kept(const RowGrid& g, int8_t* codes, float* scales) {
+    return {codes, scales, g.channels, g.nblk, g.shift, g.lanes};
+}
 int64_t row_blocks(const RowGrid& g) {
     return sg::ceil_div(g.rows, (int64_t)g.phases * g.iters) * g.tiles;
 }
@@ -130,37 +133,30 @@ __device__ __forceinline__ Place place(const RowGrid& g) {
     return p;
 }
 
-template <class T, int AW>
-__device__ __forceinline__ void keep_unit(const Raw<T>& raw, const RowGrid& g, const Place& p,
-                                          int64_t row, bool on, int8_t* codes, float* scales) {
-    float v[8];
-    unpack(raw, v);
-    const uint32_t m = block_max(on ? largest(v) : 0u, g.lanes);
-    float scale, inverse;
-    block_scale(m, scale, inverse);
-    if (!on) return;
-    st_codes<AW == 16>(codes + row * g.channels + p.unit * kUnit, encode(v, inverse), p.cnt);
-    if (p.unit % g.lanes == 0) scales[row * g.nblk + (p.unit >> g.shift)] = scale;
+// The rows of one step of a thread's loop: row0 + u*phases for u < U.
+template <int U>
+__device__ __forceinline__ void live_rows(const RowGrid& g, const Place& p, int64_t row,
+                                          bool (&live)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        live[u] = p.phase < g.phases && row + (int64_t)u * g.phases < p.end;
 }
 
 template <class T, int AW>
 __global__ void __launch_bounds__(kThreads)
-    k_pack8(int8_t* __restrict__ codes, float* __restrict__ scales, const T* __restrict__ x,
-            int64_t pitch, RowGrid g) {
+    k_pack8(Kept kept, const T* __restrict__ x, int64_t pitch, RowGrid g) {
     constexpr int U = 4;
     const Place p = place(g);
-    for (int64_t base = p.row0; base < p.end; base += (int64_t)U * g.phases) {
+    const T* at = x + p.unit * kUnit;
+    for (int64_t row = p.row0 + p.phase; row - p.phase < p.end; row += (int64_t)U * g.phases) {
+        bool live[U];
+        live_rows<U>(g, p, row, live);
         Raw<T> raw[U] = {};
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t row = base + p.phase + (int64_t)u * g.phases;
-            if (p.on && row < p.end) raw[u] = ld_unit<T, AW>(x + row * pitch + p.unit * kUnit, p.cnt);
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t row = base + p.phase + (int64_t)u * g.phases;
-            keep_unit<T, AW>(raw[u], g, p, row, p.on && row < p.end, codes, scales);
-        }
+        for (int u = 0; u < U; u++)
+            if (p.on && live[u])
+                raw[u] = ld_unit<T, AW>(at + (row + (int64_t)u * g.phases) * pitch, p.cnt);
+        keep_units<T, AW, U>(raw, kept, row, g.phases, live, p.unit, p.cnt, p.on);
     }
 }
 
@@ -186,10 +182,8 @@ __global__ void __launch_bounds__(kThreads)
         for (int u = 0; u < U; u++) {
             const int64_t row = base + (int64_t)u * g.phases;
             if (row < p.end) {
-                float v[8];
-                decode(c[u], s[u], v);
                 Raw<T> r;
-                pack(v, r);
+                pack(decode(c[u], s[u]), r);
                 st_unit<T, AW>(x + row * pitch + p.unit * kUnit, r, p.cnt);
             }
         }
@@ -201,47 +195,49 @@ __global__ void __launch_bounds__(kThreads)
 struct GatedArgs {
     void* y;
     const void *a, *b;
-    int8_t *a_codes, *b_codes;
-    float *a_scales, *b_scales;
+    Kept ka, kb;  // codes null: not kept
     int64_t a_pitch, b_pitch, y_pitch;
     int act;
     float param;
 };
 
-template <class T, int AW>
+template <class T, int AW, bool kGate, bool kKeep>
 __global__ void __launch_bounds__(kThreads) k_gated(GatedArgs k, RowGrid g) {
     constexpr int U = sizeof(T) == 2 ? 4 : 2;
     const Place p = place(g);
-    const T *a = (const T*)k.a, *b = (const T*)k.b;
-    for (int64_t base = p.row0; base < p.end; base += (int64_t)U * g.phases) {
+    const T* a = (const T*)k.a + p.unit * kUnit;
+    const T* b = (const T*)k.b + p.unit * kUnit;
+    T* y = (T*)k.y + p.unit * kUnit;
+    for (int64_t row = p.row0 + p.phase; row - p.phase < p.end; row += (int64_t)U * g.phases) {
+        bool live[U];
+        live_rows<U>(g, p, row, live);
         Raw<T> ra[U] = {}, rb[U] = {};
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t row = base + p.phase + (int64_t)u * g.phases;
-            if (p.on && row < p.end) {
-                ra[u] = ld_unit<T, AW>(a + row * k.a_pitch + p.unit * kUnit, p.cnt);
-                if (b) rb[u] = ld_unit<T, AW>(b + row * k.b_pitch + p.unit * kUnit, p.cnt);
+        for (int u = 0; u < U; u++)
+            if (p.on && live[u]) {
+                const int64_t at = row + (int64_t)u * g.phases;
+                ra[u] = ld_unit<T, AW>(a + at * k.a_pitch, p.cnt);
+                if (kGate) rb[u] = ld_unit<T, AW>(b + at * k.b_pitch, p.cnt);
             }
-        }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t row = base + p.phase + (int64_t)u * g.phases;
-            const bool on = p.on && row < p.end;
-            if (on) {
-                float v[8], w[8];
-                unpack(ra[u], v);
+        for (int u = 0; u < U; u++)
+            if (p.on && live[u]) {
+                V8 v = unpack(ra[u]);
                 activate<sizeof(T) == 2>(v, k.act, k.param);
-                if (b) {
-                    unpack(rb[u], w);
+                if (kGate) {
+                    const V8 w = unpack(rb[u]);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] *= w[i];
+                    for (int i = 0; i < 4; i++) v.p[i] = mul2(v.p[i], w.p[i]);
                 }
                 Raw<T> r;
                 pack(v, r);
-                st_unit<T, AW>((T*)k.y + row * k.y_pitch + p.unit * kUnit, r, p.cnt);
+                st_unit<T, AW>(y + (row + (int64_t)u * g.phases) * k.y_pitch, r, p.cnt);
             }
-            if (k.a_codes) keep_unit<T, AW>(ra[u], g, p, row, on, k.a_codes, k.a_scales);
-            if (k.b_codes) keep_unit<T, AW>(rb[u], g, p, row, on, k.b_codes, k.b_scales);
+        if (kKeep) {
+            if (k.ka.codes)
+                keep_units<T, AW, U>(ra, k.ka, row, g.phases, live, p.unit, p.cnt, p.on);
+            if (kGate && k.kb.codes)
+                keep_units<T, AW, U>(rb, k.kb, row, g.phases, live, p.unit, p.cnt, p.on);
         }
     }
 }
@@ -271,20 +267,14 @@ struct Source {
             raw = ld_unit<T, AW>(x + row * pitch + p.unit * kUnit, p.cnt);
         }
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        if (kFrom)
-            decode(codes, scale, v);
-        else
-            unpack(raw, v);
-    }
+    __device__ __forceinline__ V8 get() const { return kFrom ? decode(codes, scale) : unpack(raw); }
 };
 
-template <class T, int AW, bool kFrom>
+template <class T, int AW, bool kFrom, bool kGate>
 __global__ void __launch_bounds__(kThreads) k_gated_back(GatedBackArgs k, RowGrid g) {
     constexpr int U = sizeof(T) == 2 ? 4 : 2;
     const Place p = place(g);
     if (!p.on) return;
-    const bool gate = k.b || k.b_codes;
     for (int64_t base = p.row0 + p.phase; base < p.end; base += (int64_t)U * g.phases) {
         Source<T, AW, kFrom> a[U], b[U];
         Raw<T> dy[U];
@@ -294,32 +284,32 @@ __global__ void __launch_bounds__(kThreads) k_gated_back(GatedBackArgs k, RowGri
             if (row < p.end) {
                 dy[u] = ld_unit<T, AW>((const T*)k.dy + row * k.y_pitch + p.unit * kUnit, p.cnt);
                 a[u].load((const T*)k.a, k.a_codes, k.a_scales, k.a_pitch, g, p, row);
-                if (gate) b[u].load((const T*)k.b, k.b_codes, k.b_scales, k.b_pitch, g, p, row);
+                if (kGate) b[u].load((const T*)k.b, k.b_codes, k.b_scales, k.b_pitch, g, p, row);
             }
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int64_t row = base + (int64_t)u * g.phases;
             if (row < p.end) {
-                float z[8], d[8], f[8], s[8];
-                a[u].get(z);
-                unpack(dy[u], d);
-                activate_slope<sizeof(T) == 2>(z, f, s, k.act, k.param);
+                V8 f, s;
+                activate_slope<sizeof(T) == 2>(a[u].get(), f, s, k.act, k.param);
+                const V8 d = unpack(dy[u]);
                 Raw<T> r;
-                if (k.db) {
+                if (kGate && k.db) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) f[i] *= d[i];
+                    for (int i = 0; i < 4; i++) f.p[i] = mul2(f.p[i], d.p[i]);
                     pack(f, r);
                     st_unit<T, AW>((T*)k.db + row * k.db_pitch + p.unit * kUnit, r, p.cnt);
                 }
                 if (k.da) {
-                    if (gate) {
-                        b[u].get(z);
+                    V8 w = d;
+                    if (kGate) {
+                        const V8 gate = b[u].get();
 #pragma unroll
-                        for (int i = 0; i < 8; i++) d[i] *= z[i];
+                        for (int i = 0; i < 4; i++) w.p[i] = mul2(w.p[i], gate.p[i]);
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) s[i] *= d[i];
+                    for (int i = 0; i < 4; i++) s.p[i] = mul2(s.p[i], w.p[i]);
                     pack(s, r);
                     st_unit<T, AW>((T*)k.da + row * k.da_pitch + p.unit * kUnit, r, p.cnt);
                 }
@@ -406,9 +396,9 @@ int simtgo_Pack8(int8_t* codes, float* scales, const void* x, int32_t type, int6
     return by_type(type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         sg::before_launch();
-        k_pack8<T, decltype(w)::value><<<(unsigned)row_blocks(g), kThreads, 0,
-                                         (cudaStream_t)stream>>>(codes, scales, (const T*)x,
-                                                                 row_pitch, g);
+        k_pack8<T, decltype(w)::value>
+            <<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(
+                kept(g, codes, scales), (const T*)x, row_pitch, g);
         return sg::launch_status(K);
     });
 }
@@ -480,13 +470,15 @@ int simtgo_Gated(void* y, const void* a, const void* b, int8_t* a_codes, float* 
     int width = access_width(c.type, {{y, m * c.y_pitch, 0}, {a, m * c.a_pitch, 0},
                                       {b, m * c.b_pitch, 0}});
     if (ka || kb) width = with_codes(width, c.channels, {a_codes, b_codes});
-    const GatedArgs k = {y, a, b, a_codes, b_codes, a_scales, b_scales,
+    const GatedArgs k = {y, a, b, kept(g, a_codes, a_scales), kept(g, b_codes, b_scales),
                          c.a_pitch, c.b_pitch, c.y_pitch, c.act, c.act_param};
     return by_type(c.type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int AW = decltype(w)::value;
+        const auto kernel = b ? (ka || kb ? k_gated<T, AW, true, true> : k_gated<T, AW, true, false>)
+                              : (ka ? k_gated<T, AW, false, true> : k_gated<T, AW, false, false>);
         sg::before_launch();
-        k_gated<T, decltype(w)::value>
-            <<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(k, g);
+        kernel<<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(k, g);
         return sg::launch_status(K);
     });
 }
@@ -543,13 +535,11 @@ int simtgo_Gated_backward(void* da, void* db, const void* dy, const void* a, con
     return by_type(c.type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int AW = decltype(w)::value;
+        const auto kernel =
+            from ? (gate ? k_gated_back<T, AW, true, true> : k_gated_back<T, AW, true, false>)
+                 : (gate ? k_gated_back<T, AW, false, true> : k_gated_back<T, AW, false, false>);
         sg::before_launch();
-        if (from)
-            k_gated_back<T, AW, true>
-                <<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(k, g);
-        else
-            k_gated_back<T, AW, false>
-                <<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(k, g);
+        kernel<<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(k, g);
         return sg::launch_status(K);
     });
 }

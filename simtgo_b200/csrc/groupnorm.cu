@@ -1,19 +1,34 @@
 // groupnorm.cu -- group norm with an activation over channels-last batches,
 // forward and backward, with the input kept as an 8-bit checkpoint on request.
 //
-// Mathematics. A thread sums x - K and (x - K)^2 for the eight channels of its
-// unit, K being the first value it meets: the shift keeps the variance exact
-// to a few ulps however far the mean is from zero, since K is one of the
-// values that are summed. Threads, blocks and chunks of a sample are then
-// joined by counts, means and sums of squared deviations (Chan, Golub and
-// LeVeque's pairwise formula), never by raw squares; a mean stays K plus a
-// small offset until the last join, so differences of means do not cancel. The backward pass needs,
-// for each channel of a sample, A = sum dz and B = sum dz*xh: weighted and summed
-// over a group's channels they give the group's two means in dx, and summed
-// over the samples they are dbias and dweight, so one pass over x and dy serves
-// both. All joins run in a fixed order.
+// Mathematics. A thread sums x - K and (x - K)^2, K being the first value it
+// meets: the shift keeps the variance exact to a few ulps however far the mean
+// is from zero, since K is one of the values that are summed. Threads, blocks
+// and chunks of a sample are then joined by counts, means and sums of squared
+// deviations (Chan, Golub and LeVeque's pairwise formula), never by raw
+// squares; a mean stays K plus a small offset until the last join, so
+// differences of means do not cancel. The backward pass needs, for each channel
+// of a sample, A = sum dz and B = sum dz*xh: weighted and summed over a group's
+// channels they give the group's two means in dx, and summed over the samples
+// they are dbias and dweight, so one pass over x and dy serves both. All joins
+// run in a fixed order.
+//
+// Two ways through the data, both reading it once from HBM:
+//
+// - k_norm, k_norm_back: a cluster of up to eight blocks takes a slab of whole
+//   groups of one sample. Each block sums its share of the rows, keeping them in
+//   shared memory (what does not fit is read again, last rows first, from L2);
+//   the blocks exchange their sums over distributed shared memory, and each
+//   finishes its own rows. One launch, nothing in HBM between.
+// - k_stats, k_join, k_apply (and their backward forms): where too few such
+//   clusters exist to fill the GPU -- a few samples of very many positions --
+//   every SM takes a chunk of a sample's rows, the chunks' sums are joined by a
+//   small kernel, and a third pass walks the chunks from their ends, whose rows
+//   L2 still holds.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <numeric>
 #include <type_traits>
 
 #include "channels.cuh"
@@ -30,18 +45,25 @@ struct Batch {
     void* out;  // y, or dx
     const int8_t* codes_in;
     const float* scales_in;
-    int8_t* codes;
-    float* scales;
     const float *mean, *rstd;
+    float *mean_out, *rstd_out;
     const int32_t* lengths;
+    Kept kept;
     int64_t xs, xr, ys, yr, os, orow;
     int n, s, c, g, d;
-    int units, lanes, tile, tiles, phases;  // lanes: that share a checkpoint block
-    int shift, nblk;
-    int chunks;  // parts a sample's rows are cut into
+    int units, tile, tiles, phases;  // of a row, or of a slab's row
+    int slab, slabs;                 // channels of a cluster's slab, slabs of a sample
+    int chunks;                      // blocks that share a sample's rows
+    int keep;                        // iterations whose rows stay in shared memory
     int ptype, act;
     float param, eps;
 };
+
+// Rows a thread loads before it uses any: while summing, and while finishing.
+template <class T>
+constexpr int kSumRows = sizeof(T) == 2 ? 8 : 4;
+template <class T>
+constexpr int kOutRows = sizeof(T) == 2 ? 4 : 2;
 
 __device__ __forceinline__ int valid_rows(const Batch& B, int n) {
     return B.lengths ? min(max(__ldg(B.lengths + n), 0), B.s) : B.s;
@@ -52,6 +74,38 @@ __device__ __forceinline__ void chunk_rows(int len, int chunks, int k, int& r0, 
     r0 = (int)min((int64_t)k * per, (int64_t)len);
     r1 = min(r0 + per, len);
 }
+
+// ---- between blocks and grids --------------------------------------------------
+
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// The word at p's place in the shared memory of the cluster's block `rank`.
+__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+    uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
+    float v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+    return v;
+}
+// Programmatic dependent launch: the kernel before has finished; the kernel
+// after may take the SMs that are free.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// ---- sums ---------------------------------------------------------------------
+// A cell is what a thread sums together: a channel, or -- where groups are whole
+// units (kSame) -- a unit.
 
 struct Moments {  // the mean is k + off; m2: the sum of squared deviations from it
     float k, off, m2;
@@ -65,24 +119,25 @@ __device__ __forceinline__ Moments join(float na, Moments a, float nb, Moments b
 }
 
 // Joins the phases of a block's threads: red holds phase p's moments of
-// channel i at [p*width + i], cnt[p] its rows. Phase 0 ends with them all.
-__device__ void join_phases(Moments* red, float* cnt, int phases, int width, int phase, int unit8,
-                            int lead) {
+// cell i at [p*width + i], cnt[p] its count. Phase 0 ends with them all. Every
+// thread calls it, after a barrier.
+template <int E>
+__device__ void join_phases(Moments* red, float* cnt, int phases, int width, int phase, int cell) {
     float* in = cnt;
     float* out = cnt + kThreads;
     for (int m = phases; m > 1;) {
         const int h = (m + 1) / 2;
-        if (phase < h && unit8 < width) {
+        if (phase < h) {
             const bool two = phase + h < m;
             const float na = in[phase], nb = two ? in[phase + h] : 0.0f;
             if (two) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    Moments* a = red + phase * width + unit8 + i;
+                for (int i = 0; i < E; i++) {
+                    Moments* a = red + phase * width + cell + i;
                     *a = join(na, *a, nb, a[h * width]);
                 }
             }
-            if (lead) out[phase] = na + nb;
+            if (cell == 0) out[phase] = na + nb;
         }
         float* t = in;
         in = out;
@@ -92,58 +147,73 @@ __device__ void join_phases(Moments* red, float* cnt, int phases, int width, int
     }
 }
 
-// Sums of x - K and (x - K)^2 down rows r, r + step, ... < r1 of one unit.
-template <class T, int AW>
+// Moments of this thread's cells over rows r0 + phase, + phases, ... < r1;
+// keep(it, raw) is handed every row's unit. Returns the number of rows.
+template <class T, int AW, bool kSame, class F>
 __device__ __forceinline__ int unit_moments(const T* x, int64_t pitch, int r, int r1, int step,
-                                            int cnt, Moments (&out)[8]) {
-    constexpr int U = sizeof(T) == 2 ? 8 : 4;
+                                            int cnt, Moments (&out)[kSame ? 1 : 8], F&& keep) {
+    constexpr int U = kSumRows<T>, P = kSame ? 1 : 4;
     if (r >= r1) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) out[i] = {0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < (kSame ? 1 : 8); i++) out[i] = {0.0f, 0.0f, 0.0f};
         return 0;
     }
-    float k[8], s1[8] = {}, s2[8] = {};
-    unpack(ld_unit<T, AW>(x + (int64_t)r * pitch, cnt), k);
+    float2 k[P], s1[P] = {}, s2[P] = {};
     int n = 0;
-    for (; r < r1; r += U * step) {
+    bool first = true;
+    for (int it = 0; r < r1; r += U * step, it += U) {
         Raw<T> raw[U];
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (r + u * step < r1) raw[u] = ld_unit<T, AW>(x + (int64_t)(r + u * step) * pitch, cnt);
+        if (first) {
+            const V8 v = unpack(raw[0]);
+#pragma unroll
+            for (int i = 0; i < P; i++) k[i] = kSame ? both(v.p[0].x) : v.p[i];
+            first = false;
+        }
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (r + u * step < r1) {
-                float v[8];
-                unpack(raw[u], v);
+                keep(it + u, raw[u]);
+                const V8 v = unpack(raw[u]);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float dv = v[i] - k[i];
-                    s1[i] += dv;
-                    s2[i] = __fmaf_rn(dv, dv, s2[i]);
+                for (int i = 0; i < 4; i++) {
+                    const float2 dv = sub2(v.p[i], k[kSame ? 0 : i]);
+                    s1[kSame ? 0 : i] = add2(s1[kSame ? 0 : i], dv);
+                    s2[kSame ? 0 : i] = fma2(dv, dv, s2[kSame ? 0 : i]);
                 }
                 n++;
             }
     }
-    const float inv = 1.0f / (float)n;
+    if (kSame) {
+        const float a = s1[0].x + s1[0].y, q = s2[0].x + s2[0].y, m = a / (float)(8 * n);
+        const float m2 = __fmaf_rn(-m, a, q);
+        out[0] = {k[0].x, m, m2 < 0.0f ? 0.0f : m2};
+    } else {
+        const float inv = 1.0f / (float)n;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float m = s1[i] * inv;
-        out[i] = {k[i], m, fmaxf(__fmaf_rn(-m, s1[i], s2[i]), 0.0f)};
+        for (int i = 0; i < (kSame ? 1 : 8); i++) {
+            const float2 a = s1[i / 2 % P], q = s2[i / 2 % P], kk = k[i / 2 % P];
+            const float m = (i & 1 ? a.y : a.x) * inv;
+            const float m2 = __fmaf_rn(-m, i & 1 ? a.y : a.x, i & 1 ? q.y : q.x);
+            out[i] = {i & 1 ? kk.y : kk.x, m, m2 < 0.0f ? 0.0f : m2};
+        }
     }
     return n;
 }
 
-// Group moments from channel moments of equal counts: sub-warps of `lanes`
-// lanes take a group each; f(group, moments) on the sub-warp's first lane.
+// Group moments from the moments of `d` cells each of `count` values: sub-warps
+// take a group each; f(group, moments) on the sub-warp's first lane.
 template <class F>
-__device__ __forceinline__ void group_moments(const Moments* chan_m, int groups, int d, float rows,
+__device__ __forceinline__ void group_moments(const Moments* cells, int groups, int d, float count,
                                               F&& f) {
     int lanes = 1;
     while (lanes < d && lanes < 32) lanes *= 2;
     const int per = kThreads / lanes, lane = threadIdx.x % lanes;
     for (int g0 = 0; g0 < groups; g0 += per) {
         const int g = g0 + threadIdx.x / lanes;
-        const Moments* c = chan_m + (int64_t)g * d;
+        const Moments* c = cells + (int64_t)g * d;
         const float k = g < groups ? c[0].k : 0.0f;
         float off = 0.0f, m2 = 0.0f;
         if (g < groups)
@@ -153,373 +223,665 @@ __device__ __forceinline__ void group_moments(const Moments* chan_m, int groups,
         if (g < groups)
             for (int i = lane; i < d; i += lanes) {
                 const float dv = (c[i].k - k) + (c[i].off - off);
-                m2 += __fmaf_rn(rows * dv, dv, c[i].m2);
+                m2 += __fmaf_rn(count * dv, dv, c[i].m2);
             }
         for (int o = lanes / 2; o; o /= 2) m2 += __shfl_xor_sync(~0u, m2, o);
         if (g < groups && lane == 0) f(g, Moments{k, off, m2});
     }
 }
 
-// ---- forward: moments of each (chunk, sample), joined, then applied ----------
+// ---- a unit's parameters ---------------------------------------------------------
 
-template <class T, int AW>
-__global__ void __launch_bounds__(kThreads) k_stats(Batch B, Moments* __restrict__ part) {
+__device__ __forceinline__ V8 ld_params(const void* p, int type, int c0, int cnt, float fallback) {
+    V8 v;
+    float f[8];
+    if (!p) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v.p[i] = both(fallback);
+        return v;
+    }
+    const char* at = (const char*)p + (int64_t)c0 * (type == SIMTGO_F32 ? 4 : 2);
+    if (cnt == kUnit && ((uintptr_t)at & 15) == 0) {
+        if (type == SIMTGO_F32) return unpack(ld_unit<float, 16>((const float*)at, 8));
+        if (type == SIMTGO_BF16)
+            return unpack(ld_unit<__nv_bfloat16, 16>((const __nv_bfloat16*)at, 8));
+        return unpack(ld_unit<__half, 16>((const __half*)at, 8));
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = i < cnt ? ld_param(p, type, c0 + i) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v.p[i] = make_float2(f[2 * i], f[2 * i + 1]);
+    return v;
+}
+
+// One value per group, spread over a unit's channels.
+template <bool kSame>
+struct PerGroup {
+    float2 v[kSame ? 1 : 4];
+    __device__ __forceinline__ float2 operator[](int i) const { return v[kSame ? 0 : i]; }
+};
+// f(group) for each of the unit's channels.
+template <bool kSame, class F>
+__device__ __forceinline__ PerGroup<kSame> per_group(int c0, int last, int d, F&& f) {
+    PerGroup<kSame> r;
+    if (kSame) {
+        r.v[0] = both(f(c0 / d));
+    } else {
+#pragma unroll
+        for (int i = 0; i < (kSame ? 1 : 4); i++)
+            r.v[i] = make_float2(f(min(c0 + 2 * i, last) / d), f(min(c0 + 2 * i + 1, last) / d));
+    }
+    return r;
+}
+
+// ---- finishing rows, forward -----------------------------------------------------------
+
+// y (and the checkpoint) of rows [r0, r1) of this thread's unit, last rows
+// first; rows of iterations below B.keep come from `kept_rows`.
+template <class T, int AW, bool kSame, bool kKeep>
+__device__ __forceinline__ void apply_rows(const Batch& B, int n, int r0, int r1, int phase,
+                                           int unit, int cnt, bool on, const PerGroup<kSame>& mean,
+                                           const V8& scale, const V8& bias,
+                                           const Raw<T>* kept_rows) {
+    constexpr int U = kOutRows<T>;
+    const T* x = (const T*)B.x + (int64_t)n * B.xs + unit * kUnit;
+    T* y = (T*)B.out + (int64_t)n * B.os + unit * kUnit;
+    const int iters = (r1 - r0 + B.phases - 1) / B.phases;
+    for (int it = (iters - 1) / U * U; it >= 0 && iters > 0; it -= U) {
+        const int row = r0 + phase + it * B.phases;
+        bool live[U];
+        Raw<T> raw[U] = {};
+#pragma unroll
+        for (int u = 0; u < U; u++) live[u] = phase < B.phases && row + u * B.phases < r1;
+        if (it + U <= B.keep) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (on && live[u]) raw[u] = kept_rows[(it + u) * kThreads + threadIdx.x];
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (on && live[u])
+                    raw[u] = ld_unit<T, AW>(x + (int64_t)(row + u * B.phases) * B.xr, cnt);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (on && live[u]) {
+                V8 v = unpack(raw[u]);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    v.p[i] = fma2(sub2(v.p[i], mean[i]), scale.p[i], bias.p[i]);
+                activate<sizeof(T) == 2>(v, B.act, B.param);
+                Raw<T> o;
+                pack(v, o);
+                st_unit<T, AW>(y + (int64_t)(row + u * B.phases) * B.orow, o, cnt);
+            }
+        if (kKeep)
+            keep_units<T, AW, U>(raw, B.kept, (int64_t)n * B.s + row, B.phases, live, unit, cnt,
+                                 on);
+    }
+}
+
+// ---- forward in one launch: a cluster per slab of a sample -------------------------------
+
+template <class T, int AW, bool kSame, bool kKeep>
+__global__ void __launch_bounds__(kThreads, 2) k_norm(Batch B) {
+    constexpr int E = kSame ? 1 : 8;
+    extern __shared__ uint4 dyn[];
+    __shared__ float cnt_sm[2 * kThreads];
+    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile, width = B.tile * E;
+    Raw<T>* rows_sm = reinterpret_cast<Raw<T>*>(dyn);
+    float2* stat = reinterpret_cast<float2*>(rows_sm + B.keep * kThreads);  // mean, rstd
+    Moments* red = reinterpret_cast<Moments*>(stat + B.slab / B.d);
+    Moments* own = red + B.phases * width;                                  // this block's groups
+
+    const int rank = (int)cluster_rank();
+    const int id = blockIdx.x / B.chunks, n = id / B.slabs, c0 = id % B.slabs * B.slab;
+    const int cw = min(B.slab, B.c - c0), groups = cw / B.d, g0 = c0 / B.d;
+    const int len = valid_rows(B, n);
+    int r0, r1;
+    chunk_rows(len, B.chunks, rank, r0, r1);
+    const int unit = c0 / kUnit + u, cnt = min(kUnit, c0 + cw - unit * kUnit);
+    const bool on = phase < B.phases && u * kUnit < cw;
+
+    Moments m[E] = {};
+    int rows = 0;
+    if (on)
+        rows = unit_moments<T, AW, kSame>(
+            (const T*)B.x + (int64_t)n * B.xs + unit * kUnit, B.xr, r0 + phase, r1, B.phases, cnt,
+            m, [&](int it, const Raw<T>& raw) {
+                if (it < B.keep) rows_sm[it * kThreads + threadIdx.x] = raw;
+            });
+    V8 scale = ld_params(on ? B.w : nullptr, B.ptype, unit * kUnit, cnt, 1.0f);
+    const V8 bias = ld_params(on ? B.b : nullptr, B.ptype, unit * kUnit, cnt, 0.0f);
+    if (phase < B.phases) {
+#pragma unroll
+        for (int i = 0; i < E; i++) red[phase * width + u * E + i] = m[i];
+        if (u == 0) cnt_sm[phase] = (float)(rows * (kSame ? kUnit : 1));
+    }
+    __syncthreads();
+    join_phases<E>(red, cnt_sm, B.phases, width, phase, u * E);
+    const int cells = kSame ? B.d / kUnit : B.d, per = kSame ? kUnit : 1;
+    group_moments(red, groups, cells, (float)(r1 - r0) * per,
+                  [&](int g, Moments q) { own[g] = q; });
+    cluster_arrive();
+    cluster_wait();
+    for (int g = threadIdx.x; g < groups; g += kThreads) {
+        Moments q = {0.0f, 0.0f, 0.0f};
+        float have = 0.0f;
+        for (int k = 0; k < B.chunks; k++) {
+            int a, b;
+            chunk_rows(len, B.chunks, k, a, b);
+            const float c = (float)(b - a) * (float)B.d;
+            const Moments o = {ld_cluster(&own[g].k, k), ld_cluster(&own[g].off, k),
+                               ld_cluster(&own[g].m2, k)};
+            if (c > 0.0f) q = join(have, q, c, o);
+            have += c;
+        }
+        const float mu = q.k + q.off, var = have > 0.0f ? q.m2 / have : 0.0f;
+        const float rs = __fdiv_rn(1.0f, __fsqrt_rn(var + B.eps));
+        stat[g] = make_float2(mu, rs);
+        if (rank == 0) {
+            const int64_t at = (int64_t)n * B.g + g0 + g;
+            if (B.mean_out) B.mean_out[at] = mu;
+            if (B.rstd_out) B.rstd_out[at] = rs;
+        }
+    }
+    cluster_arrive();  // the others' shared memory has been read
+    __syncthreads();
+    const int last = c0 + cw - 1, first = min(unit * kUnit, last);
+    const auto mean = per_group<kSame>(first, last, B.d, [&](int g) { return stat[g - g0].x; });
+    const auto rstd = per_group<kSame>(first, last, B.d, [&](int g) { return stat[g - g0].y; });
+#pragma unroll
+    for (int i = 0; i < 4; i++) scale.p[i] = mul2(scale.p[i], rstd[i]);
+    apply_rows<T, AW, kSame, kKeep>(B, n, r0, r1, phase, unit, cnt, on, mean, scale, bias, rows_sm);
+    cluster_wait();
+}
+
+// ---- forward over chunks: moments, joined, then applied ---------------------------
+
+template <class T, int AW, bool kSame>
+__global__ void __launch_bounds__(kThreads, 2) k_stats(Batch B, Moments* __restrict__ part) {
+    constexpr int E = kSame ? 1 : 8;
     extern __shared__ Moments sm[];
-    __shared__ float cnt[2 * kThreads];
-    Moments* chan_m = sm;                              // B.c, rounded up to units
-    Moments* red = sm + (int64_t)B.units * kUnit;      // phases * tile * 8
+    __shared__ float cnt_sm[2 * kThreads];
+    Moments* cell_m = sm;                         // every cell of the row
+    Moments* red = sm + (int64_t)B.units * E;     // phases * tile * E
     const int n = blockIdx.x / B.chunks, k = blockIdx.x % B.chunks;
     int r0, r1;
     chunk_rows(valid_rows(B, n), B.chunks, k, r0, r1);
     const T* x = (const T*)B.x + (int64_t)n * B.xs;
-    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
+    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile, width = B.tile * E;
     for (int t = 0; t < B.tiles; t++) {
-        const int unit = t * B.tile + u, width = B.tile * kUnit;
+        const int unit = t * B.tile + u;
         if (phase < B.phases) {
-            Moments m[8] = {};
+            Moments m[E] = {};
             int rows = 0;
             if (unit < B.units)
-                rows = unit_moments<T, AW>(x + unit * kUnit, B.xr, r0 + phase, r1, B.phases,
-                                           min(kUnit, B.c - unit * kUnit), m);
+                rows = unit_moments<T, AW, kSame>(x + unit * kUnit, B.xr, r0 + phase, r1, B.phases,
+                                                  min(kUnit, B.c - unit * kUnit), m,
+                                                  [](int, const Raw<T>&) {});
 #pragma unroll
-            for (int i = 0; i < 8; i++) red[phase * width + u * 8 + i] = m[i];
-            if (u == 0) cnt[phase] = (float)rows;
+            for (int i = 0; i < E; i++) red[phase * width + u * E + i] = m[i];
+            if (u == 0) cnt_sm[phase] = (float)(rows * (kSame ? kUnit : 1));
         }
         __syncthreads();
-        join_phases(red, cnt, B.phases, width, phase, u * 8, u == 0);
+        join_phases<E>(red, cnt_sm, B.phases, width, phase, u * E);
         if (phase == 0 && unit < B.units) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) chan_m[unit * kUnit + i] = red[u * 8 + i];
+            for (int i = 0; i < E; i++) cell_m[unit * E + i] = red[u * E + i];
         }
         __syncthreads();
     }
+    grid_release();
     Moments* o = part + ((int64_t)n * B.chunks + k) * B.g;
-    group_moments(chan_m, B.g, B.d, (float)(r1 - r0), [&](int g, Moments m) { o[g] = m; });
+    group_moments(cell_m, B.g, kSame ? B.d / kUnit : B.d, (float)(r1 - r0) * (kSame ? kUnit : 1),
+                  [&](int g, Moments m) { o[g] = m; });
 }
 
-// One warp per (sample, group) joins the chunks, in double.
-__global__ void __launch_bounds__(kThreads)
-    k_join(Batch B, const Moments* __restrict__ part, float* __restrict__ mean,
-           float* __restrict__ rstd) {
-    const int64_t id = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 32;
-    const int lane = threadIdx.x % 32;
-    if (id >= (int64_t)B.n * B.g) return;
-    const int n = (int)(id / B.g), g = (int)(id % B.g);
+// A block joins the chunks of up to `wide` groups of a sample: its threads take
+// wide groups by kJoin/wide chunks at a time. In double, about the first
+// chunk's mean, so one pass over the parts serves both moments.
+constexpr int kJoin = 512;
+__global__ void __launch_bounds__(kJoin)
+    k_join(Batch B, const Moments* __restrict__ part, int wide, int blocks) {
+    __shared__ double s1[kJoin], s2[kJoin];
+    grid_wait();
+    const int n = blockIdx.x / blocks, g = blockIdx.x % blocks * wide + threadIdx.x % wide;
+    const int lane = threadIdx.x / wide, lanes = kJoin / wide;
     const int len = valid_rows(B, n);
-    const Moments* p = part + (int64_t)n * B.chunks * B.g + g;
-    const double count = (double)len * B.d;
-    double mu = 0.0, m2 = 0.0;
-    for (int k = lane; k < B.chunks; k += 32) {
-        int r0, r1;
-        chunk_rows(len, B.chunks, k, r0, r1);
-        const Moments q = p[(int64_t)k * B.g];
-        mu += (double)(r1 - r0) * B.d * ((double)q.k + q.off);
+    double a = 0.0, q = 0.0, ref = 0.0;
+    if (g < B.g) {
+        const Moments* p = part + (int64_t)n * B.chunks * B.g + g;
+        ref = (double)p[0].k + p[0].off;
+#pragma unroll 4
+        for (int k = lane; k < B.chunks; k += lanes) {
+            int r0, r1;
+            chunk_rows(len, B.chunks, k, r0, r1);
+            const Moments m = p[(int64_t)k * B.g];
+            const double c = (double)(r1 - r0) * B.d, dv = ((double)m.k + m.off) - ref;
+            if (r1 > r0) {
+                a += c * dv;
+                q += m.m2 + c * dv * dv;
+            }
+        }
     }
-    for (int o = 16; o; o /= 2) mu += __shfl_xor_sync(~0u, mu, o);
-    mu = len ? mu / count : 0.0;
-    for (int k = lane; k < B.chunks; k += 32) {
-        int r0, r1;
-        chunk_rows(len, B.chunks, k, r0, r1);
-        const Moments q = p[(int64_t)k * B.g];
-        const double dv = (double)q.k + q.off - mu;
-        m2 += q.m2 + (double)(r1 - r0) * B.d * dv * dv;
+    s1[threadIdx.x] = a;
+    s2[threadIdx.x] = q;
+    __syncthreads();
+    for (int h = lanes / 2; h; h /= 2) {
+        if (lane < h) {
+            s1[threadIdx.x] += s1[threadIdx.x + h * wide];
+            s2[threadIdx.x] += s2[threadIdx.x + h * wide];
+        }
+        __syncthreads();
     }
-    for (int o = 16; o; o /= 2) m2 += __shfl_xor_sync(~0u, m2, o);
-    if (lane == 0) {
-        mean[id] = (float)mu;
-        rstd[id] = (float)(1.0 / sqrt((len ? m2 / count : 0.0) + (double)B.eps));
-    }
-}
-
-// The eight channels' parameters of a unit.
-struct Params {
-    float mean[8], rstd[8], w[8], b[8];
-};
-__device__ __forceinline__ void load_params(const Batch& B, int n, int unit, Params& q) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int c = min(unit * kUnit + i, B.c - 1);
-        const int64_t g = (int64_t)n * B.g + c / B.d;
-        q.mean[i] = __ldg(B.mean + g);
-        q.rstd[i] = __ldg(B.rstd + g);
-        q.w[i] = B.w ? ld_param(B.w, B.ptype, c) : 1.0f;
-        q.b[i] = B.b ? ld_param(B.b, B.ptype, c) : 0.0f;
+    grid_release();
+    if (lane == 0 && g < B.g) {
+        const double count = (double)len * B.d;
+        const double off = len ? s1[threadIdx.x] / count : 0.0;
+        const double var = len ? s2[threadIdx.x] / count - off * off : 0.0;
+        const int64_t at = (int64_t)n * B.g + g;
+        B.mean_out[at] = len ? (float)(ref + off) : 0.0f;
+        B.rstd_out[at] = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)B.eps));
     }
 }
 
-template <class T, int AW>
-__device__ __forceinline__ void keep_row(const Batch& B, const Raw<T>& raw, int64_t row, int unit,
-                                         int cnt, bool on) {
-    float v[8];
-    unpack(raw, v);
-    const uint32_t m = block_max(on ? largest(v) : 0u, B.lanes);
-    float scale, inverse;
-    block_scale(m, scale, inverse);
-    if (!on) return;
-    st_codes<AW == 16>(B.codes + row * B.c + unit * kUnit, encode(v, inverse), cnt);
-    if (unit % B.lanes == 0) B.scales[row * B.nblk + (unit >> B.shift)] = scale;
-}
-
-template <class T, int AW>
-__global__ void __launch_bounds__(kThreads) k_apply(Batch B) {
-    constexpr int U = sizeof(T) == 2 ? 4 : 2;
-    const int n = blockIdx.x / B.chunks;
+template <class T, int AW, bool kSame, bool kKeep>
+__global__ void __launch_bounds__(kThreads, 2) k_apply(Batch B) {
+    grid_wait();
+    const int id = gridDim.x - 1 - blockIdx.x, n = id / B.chunks;
     int r0, r1;
-    chunk_rows(valid_rows(B, n), B.chunks, blockIdx.x % B.chunks, r0, r1);
+    chunk_rows(valid_rows(B, n), B.chunks, id % B.chunks, r0, r1);
     if (r0 >= r1) return;
-    const T* x = (const T*)B.x + (int64_t)n * B.xs;
-    T* y = (T*)B.out + (int64_t)n * B.os;
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
+    const float *mu = B.mean_out + (int64_t)n * B.g, *rs = B.rstd_out + (int64_t)n * B.g;
     for (int t = 0; t < B.tiles; t++) {
         const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
         const bool on = phase < B.phases && unit < B.units;
-        Params q;
-        if (on) load_params(B, n, unit, q);
+        const int first = min(unit * kUnit, B.c - 1);
+        const auto mean = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return mu[g]; });
+        const auto rstd = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return rs[g]; });
+        V8 scale = ld_params(on ? B.w : nullptr, B.ptype, unit * kUnit, cnt, 1.0f);
+        const V8 bias = ld_params(on ? B.b : nullptr, B.ptype, unit * kUnit, cnt, 0.0f);
 #pragma unroll
-        for (int i = 0; i < 8; i++) q.w[i] *= q.rstd[i];
-        for (int base = r0; base < r1; base += U * B.phases) {
-            Raw<T> raw[U] = {};
-#pragma unroll
-            for (int j = 0; j < U; j++) {
-                const int r = base + phase + j * B.phases;
-                if (on && r < r1)
-                    raw[j] = ld_unit<T, AW>(x + (int64_t)r * B.xr + unit * kUnit, cnt);
-            }
-#pragma unroll
-            for (int j = 0; j < U; j++) {
-                const int r = base + phase + j * B.phases;
-                if (on && r < r1) {
-                    float v[8];
-                    unpack(raw[j], v);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = __fmaf_rn(v[i] - q.mean[i], q.w[i], q.b[i]);
-                    activate<sizeof(T) == 2>(v, B.act, B.param);
-                    Raw<T> o;
-                    pack(v, o);
-                    st_unit<T, AW>(y + (int64_t)r * B.orow + unit * kUnit, o, cnt);
-                }
-                if (B.codes)
-                    keep_row<T, AW>(B, raw[j], (int64_t)n * B.s + r, unit, cnt, on && r < r1);
-            }
-        }
+        for (int i = 0; i < 4; i++) scale.p[i] = mul2(scale.p[i], rstd[i]);
+        apply_rows<T, AW, kSame, kKeep>(B, n, r0, r1, phase, unit, cnt, on, mean, scale, bias,
+                                        nullptr);
     }
 }
 
 // ---- backward ---------------------------------------------------------------------
 
-// A unit of x: from the tensor, or from its checkpoint.
+// A unit of x and of dy, x from the tensor or from its checkpoint.
 template <class T, int AW, bool kFrom>
-struct Input {
-    Raw<T> raw;
+struct Pair {
+    Raw<T> dy, x;
     Codes codes;
     float scale;
     __device__ __forceinline__ void load(const Batch& B, int n, int r, int unit, int cnt) {
+        dy = ld_unit<T, AW>((const T*)B.dy + (int64_t)n * B.ys + (int64_t)r * B.yr + unit * kUnit,
+                            cnt);
         if (kFrom) {
             const int64_t row = (int64_t)n * B.s + r;
             codes = ld_codes<AW == 16>(B.codes_in + row * B.c + unit * kUnit, cnt);
-            scale = __ldg(B.scales_in + row * B.nblk + (unit >> B.shift));
+            scale = __ldg(B.scales_in + row * B.kept.nblk + (unit >> B.kept.shift));
         } else {
-            raw = ld_unit<T, AW>((const T*)B.x + (int64_t)n * B.xs + (int64_t)r * B.xr + unit * kUnit,
-                                 cnt);
+            x = ld_unit<T, AW>((const T*)B.x + (int64_t)n * B.xs + (int64_t)r * B.xr + unit * kUnit,
+                               cnt);
         }
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        if (kFrom)
-            decode(codes, scale, v);
-        else
-            unpack(raw, v);
+    __device__ __forceinline__ V8 input() const { return kFrom ? decode(codes, scale) : unpack(x); }
+};
+// The same in shared memory: arrays of iterations by threads.
+template <class T, bool kFrom>
+struct PairStore {
+    Raw<T>* dy;
+    Raw<T>* x;
+    uint2* codes;
+    float* scale;
+    static constexpr int kBytes = (int)sizeof(Raw<T>) + (kFrom ? 12 : (int)sizeof(Raw<T>));
+    __device__ __forceinline__ PairStore(void* base, int iters) {
+        char* p = (char*)base;
+        const int64_t cells = (int64_t)iters * kThreads;
+        dy = (Raw<T>*)p;
+        x = (Raw<T>*)(p + cells * sizeof(Raw<T>));
+        codes = (uint2*)x;
+        scale = (float*)(codes + cells);
+    }
+    template <int AW>
+    __device__ __forceinline__ void put(int it, const Pair<T, AW, kFrom>& v) {
+        const int at = it * kThreads + threadIdx.x;
+        dy[at] = v.dy;
+        if (kFrom) {
+            codes[at] = v.codes.q;
+            scale[at] = v.scale;
+        } else {
+            x[at] = v.x;
+        }
+    }
+    template <int AW>
+    __device__ __forceinline__ void get(int it, Pair<T, AW, kFrom>& v) const {
+        const int at = it * kThreads + threadIdx.x;
+        v.dy = dy[at];
+        if (kFrom) {
+            v.codes.q = codes[at];
+            v.scale = scale[at];
+        } else {
+            v.x = x[at];
+        }
     }
 };
 
-// xh and dz = dy * act'(z) of one unit.
-template <class T>
-__device__ __forceinline__ void slopes(const Batch& B, const Params& q, const Raw<T>& dy,
-                                       float (&xh)[8], float (&dz)[8]) {
-    float z[8], f[8], s[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        xh[i] = (xh[i] - q.mean[i]) * q.rstd[i];
-        z[i] = __fmaf_rn(xh[i], q.w[i], q.b[i]);
-    }
-    activate_slope<sizeof(T) == 2>(z, f, s, B.act, B.param);
-    unpack(dy, dz);
-#pragma unroll
-    for (int i = 0; i < 8; i++) dz[i] *= s[i];
+template <bool kSame>
+struct BackParams {
+    PerGroup<kSame> mean, rstd;
+    V8 w, b;
+};
+template <bool kSame>
+__device__ __forceinline__ BackParams<kSame> back_params(const Batch& B, int n, int unit, int cnt,
+                                                         bool on) {
+    BackParams<kSame> q;
+    const int first = min(unit * kUnit, B.c - 1);
+    const float *mu = B.mean + (int64_t)n * B.g, *rs = B.rstd + (int64_t)n * B.g;
+    q.mean = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return __ldg(mu + g); });
+    q.rstd = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return __ldg(rs + g); });
+    q.w = ld_params(on ? B.w : nullptr, B.ptype, unit * kUnit, cnt, 1.0f);
+    q.b = ld_params(on ? B.b : nullptr, B.ptype, unit * kUnit, cnt, 0.0f);
+    return q;
 }
 
-// A = sum dz and B = sum dz*xh of every channel of a chunk.
-template <class T, int AW, bool kFrom>
-__global__ void __launch_bounds__(kThreads) k_back_stats(Batch B, float2* __restrict__ part) {
-    extern __shared__ float2 red2[];
-    constexpr int U = sizeof(T) == 2 ? 4 : 2;
+// xh and dz = dy * act'(z) of one unit.
+template <class T, int AW, bool kFrom, bool kSame>
+__device__ __forceinline__ void slopes(const Batch& B, const BackParams<kSame>& q,
+                                       const Pair<T, AW, kFrom>& in, V8& xh, V8& dz) {
+    V8 z, f;
+    xh = in.input();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        xh.p[i] = mul2(sub2(xh.p[i], q.mean[i]), q.rstd[i]);
+        z.p[i] = fma2(xh.p[i], q.w.p[i], q.b.p[i]);
+    }
+    const V8 g = unpack(in.dy);
+    if (B.act == SIMTGO_ACT_NONE) {
+        dz = g;
+        return;
+    }
+    activate_slope<sizeof(T) == 2>(z, f, dz, B.act, B.param);
+#pragma unroll
+    for (int i = 0; i < 4; i++) dz.p[i] = mul2(dz.p[i], g.p[i]);
+}
+
+// Sums A = dz and C = dz*xh of the unit's channels over the thread's rows.
+template <class T, int AW, bool kFrom, bool kSame, class F>
+__device__ __forceinline__ void back_sums(const Batch& B, const BackParams<kSame>& q, int n, int r,
+                                          int r1, int unit, int cnt, float2 (&a)[4], float2 (&c)[4],
+                                          F&& keep) {
+    constexpr int U = kOutRows<T>;
+    for (int it = 0; r < r1; r += U * B.phases, it += U) {
+        Pair<T, AW, kFrom> in[U];
+#pragma unroll
+        for (int j = 0; j < U; j++)
+            if (r + j * B.phases < r1) in[j].load(B, n, r + j * B.phases, unit, cnt);
+#pragma unroll
+        for (int j = 0; j < U; j++)
+            if (r + j * B.phases < r1) {
+                keep(it + j, in[j]);
+                V8 xh, dz;
+                slopes(B, q, in[j], xh, dz);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    a[i] = add2(a[i], dz.p[i]);
+                    c[i] = fma2(dz.p[i], xh.p[i], c[i]);
+                }
+            }
+    }
+}
+
+// Adds the phases' (A, B) of every channel; phase 0 ends with the sums. Every
+// thread calls it; it begins with a barrier.
+__device__ __forceinline__ void add_phases(float2* red, int phases, int width, int phase, int u,
+                                           const float2 (&a)[4], const float2 (&b)[4]) {
+    // (A, A, B, B) of two channels at a time: 16 bytes a thread.
+    float4* mine = reinterpret_cast<float4*>(red + phase * width) + u * 4;
+    if (phase < phases) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) mine[i] = make_float4(a[i].x, a[i].y, b[i].x, b[i].y);
+    }
+    __syncthreads();
+    for (int m = phases; m > 1;) {
+        const int h = (m + 1) / 2;
+        if (phase + h < m) {
+            const float4* o = reinterpret_cast<const float4*>(red + (phase + h) * width) + u * 4;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4 v = o[i], w = mine[i];
+                mine[i] = make_float4(w.x + v.x, w.y + v.y, w.z + v.z, w.w + v.w);
+            }
+        }
+        m = h;
+        __syncthreads();
+    }
+}
+// Channel i's (A, B) after add_phases.
+__device__ __forceinline__ float2 channel_sum(const float2* red, int i) {
+    const float4 v = reinterpret_cast<const float4*>(red)[i / 2];
+    return i & 1 ? make_float2(v.y, v.w) : make_float2(v.x, v.z);
+}
+
+// sum of w*A and w*B over each group's d channels, at(i) giving channel i's
+// (A, B): f(group, sums) on the first lane of a sub-warp.
+template <class At, class F>
+__device__ __forceinline__ void group_sums(const Batch& B, int c0, int groups, At&& at, F&& f) {
+    int lanes = 1;
+    while (lanes < B.d && lanes < 32) lanes *= 2;
+    const int per = kThreads / lanes, lane = threadIdx.x % lanes;
+    for (int g0 = 0; g0 < groups; g0 += per) {
+        const int g = g0 + threadIdx.x / lanes;
+        float x = 0.0f, y = 0.0f;
+        if (g < groups)
+            for (int i = lane; i < B.d; i += lanes) {
+                const float2 v = at(g * B.d + i);
+                const float w = B.w ? ld_param(B.w, B.ptype, c0 + g * B.d + i) : 1.0f;
+                x = __fmaf_rn(w, v.x, x);
+                y = __fmaf_rn(w, v.y, y);
+            }
+        for (int o = lanes / 2; o; o /= 2) {
+            x += __shfl_xor_sync(~0u, x, o);
+            y += __shfl_xor_sync(~0u, y, o);
+        }
+        if (g < groups && lane == 0) f(g, make_float2(x, y));
+    }
+}
+
+// dx of rows [r0, r1) of this thread's unit, last rows first.
+template <class T, int AW, bool kFrom, bool kSame>
+__device__ __forceinline__ void back_rows(const Batch& B, const BackParams<kSame>& q,
+                                          const PerGroup<kSame>& s1, const PerGroup<kSame>& s2,
+                                          int n, int r0, int r1, int phase, int unit, int cnt,
+                                          const PairStore<T, kFrom>& store) {
+    constexpr int U = kOutRows<T>;
+    T* dx = (T*)B.out + (int64_t)n * B.os + unit * kUnit;
+    const int iters = (r1 - r0 - phase + B.phases - 1) / B.phases;
+    for (int it = (iters - 1) / U * U; it >= 0 && iters > 0; it -= U) {
+        const int row = r0 + phase + it * B.phases;
+        Pair<T, AW, kFrom> in[U];
+        if (it + U <= B.keep) {
+#pragma unroll
+            for (int j = 0; j < U; j++)
+                if (row + j * B.phases < r1) store.get(it + j, in[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < U; j++)
+                if (row + j * B.phases < r1) in[j].load(B, n, row + j * B.phases, unit, cnt);
+        }
+#pragma unroll
+        for (int j = 0; j < U; j++)
+            if (row + j * B.phases < r1) {
+                V8 xh, dz;
+                slopes(B, q, in[j], xh, dz);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 v = fma2(dz.p[i], q.w.p[i], neg2(s1[i]));
+                    dz.p[i] = mul2(q.rstd[i], fma2(neg2(xh.p[i]), s2[i], v));
+                }
+                Raw<T> o;
+                pack(dz, o);
+                st_unit<T, AW>(dx + (int64_t)(row + j * B.phases) * B.orow, o, cnt);
+            }
+    }
+}
+
+// One launch for dx: a cluster per slab of a sample. part, where wanted,
+// receives every block's (A, B) of its channels, for k_back_join.
+template <class T, int AW, bool kFrom, bool kSame>
+__global__ void __launch_bounds__(kThreads, 2) k_norm_back(Batch B, float2* __restrict__ part) {
+    extern __shared__ uint4 dyn[];
+    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile, width = B.tile * kUnit;
+    PairStore<T, kFrom> store(dyn, B.keep);
+    float2* red = reinterpret_cast<float2*>(
+        (char*)dyn + (int64_t)B.keep * kThreads * PairStore<T, kFrom>::kBytes);
+    float2* own = red + B.phases * width;     // this block's group sums
+    float2* means = own + B.slab / B.d;       // the cluster's, over the count
+
+    const int rank = (int)cluster_rank();
+    const int id = blockIdx.x / B.chunks, n = id / B.slabs, c0 = id % B.slabs * B.slab;
+    const int cw = min(B.slab, B.c - c0), groups = cw / B.d, g0 = c0 / B.d;
+    const int len = valid_rows(B, n);
+    int r0, r1;
+    chunk_rows(len, B.chunks, rank, r0, r1);
+    const int unit = c0 / kUnit + u, cnt = min(kUnit, c0 + cw - unit * kUnit);
+    const bool on = phase < B.phases && u * kUnit < cw;
+
+    const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, on);
+    float2 a[4] = {}, b[4] = {};
+    if (on)
+        back_sums<T, AW, kFrom>(B, q, n, r0 + phase, r1, unit, cnt, a, b,
+                                [&](int it, const Pair<T, AW, kFrom>& v) {
+                                    if (it < B.keep) store.put(it, v);
+                                });
+    add_phases(red, B.phases, width, phase, u, a, b);
+    if (part)
+        for (int i = threadIdx.x; i < cw; i += kThreads)
+            part[((int64_t)n * B.chunks + rank) * B.c + c0 + i] = channel_sum(red, i);
+    grid_release();
+    if (!B.out) return;  // the same for every block of the grid
+    group_sums(B, c0, groups, [&](int i) { return channel_sum(red, i); },
+               [&](int g, float2 v) { own[g] = v; });
+    cluster_arrive();
+    cluster_wait();
+    for (int g = threadIdx.x; g < groups; g += kThreads) {
+        float x = 0.0f, y = 0.0f;
+        for (int k = 0; k < B.chunks; k++) {
+            x += ld_cluster(&own[g].x, k);
+            y += ld_cluster(&own[g].y, k);
+        }
+        const float inv = len ? 1.0f / ((float)len * (float)B.d) : 0.0f;
+        means[g] = make_float2(x * inv, y * inv);
+    }
+    cluster_arrive();
+    __syncthreads();
+    if (on) {
+        const int last = c0 + cw - 1, first = min(unit * kUnit, last);
+        const auto s1 = per_group<kSame>(first, last, B.d, [&](int g) { return means[g - g0].x; });
+        const auto s2 = per_group<kSame>(first, last, B.d, [&](int g) { return means[g - g0].y; });
+        back_rows<T, AW, kFrom, kSame>(B, q, s1, s2, n, r0, r1, phase, unit, cnt, store);
+    }
+    cluster_wait();
+}
+
+// Over chunks: (A, B) of every channel of a chunk.
+template <class T, int AW, bool kFrom, bool kSame>
+__global__ void __launch_bounds__(kThreads, 2) k_back_stats(Batch B, float2* __restrict__ part) {
+    extern __shared__ float4 red4[];
+    float2* red = reinterpret_cast<float2*>(red4);
     const int n = blockIdx.x / B.chunks, k = blockIdx.x % B.chunks;
     int r0, r1;
     chunk_rows(valid_rows(B, n), B.chunks, k, r0, r1);
-    const T* dy = (const T*)B.dy + (int64_t)n * B.ys;
     float2* o = part + ((int64_t)n * B.chunks + k) * B.c;
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile, width = B.tile * kUnit;
     for (int t = 0; t < B.tiles; t++) {
         const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
         const bool on = phase < B.phases && unit < B.units;
-        float a[8] = {}, b[8] = {};
+        float2 a[4] = {}, b[4] = {};
         if (on && r0 < r1) {
-            Params q;
-            load_params(B, n, unit, q);
-            for (int r = r0 + phase; r < r1; r += U * B.phases) {
-                Raw<T> g[U];
-                Input<T, AW, kFrom> x[U];
-#pragma unroll
-                for (int j = 0; j < U; j++) {
-                    const int rr = r + j * B.phases;
-                    if (rr < r1) {
-                        g[j] = ld_unit<T, AW>(dy + (int64_t)rr * B.yr + unit * kUnit, cnt);
-                        x[j].load(B, n, rr, unit, cnt);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < U; j++)
-                    if (r + j * B.phases < r1) {
-                        float xh[8], dz[8];
-                        x[j].get(xh);
-                        slopes(B, q, g[j], xh, dz);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            a[i] += dz[i];
-                            b[i] = __fmaf_rn(dz[i], xh[i], b[i]);
-                        }
-                    }
-            }
+            const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, on);
+            back_sums<T, AW, kFrom>(B, q, n, r0 + phase, r1, unit, cnt, a, b,
+                                    [](int, const Pair<T, AW, kFrom>&) {});
         }
-        if (phase < B.phases) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) red2[phase * width + u * 8 + i] = make_float2(a[i], b[i]);
-        }
-        __syncthreads();
-        for (int m = B.phases; m > 1;) {
-            const int h = (m + 1) / 2;
-            if (phase + h < m) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    float2* p = red2 + phase * width + u * 8 + i;
-                    const float2 w = p[h * width];
-                    p->x += w.x;
-                    p->y += w.y;
-                }
-            }
-            m = h;
-            __syncthreads();
-        }
-        if (phase == 0 && unit < B.units) {
-            for (int i = 0; i < cnt; i++) o[unit * kUnit + i] = red2[u * 8 + i];
-        }
+        add_phases(red, B.phases, width, phase, u, a, b);
+        const int c0 = t * width;
+        for (int i = threadIdx.x; i < min(width, B.c - c0); i += kThreads)
+            o[c0 + i] = channel_sum(red, i);
         __syncthreads();
     }
+    grid_release();
 }
 
-// One warp per (sample, group): its means of dz*w and dz*w*xh.
-__global__ void __launch_bounds__(kThreads)
-    k_back_groups(Batch B, const float2* __restrict__ part, float2* __restrict__ means) {
-    const int64_t id = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 32;
-    const int lane = threadIdx.x % 32;
-    if (id >= (int64_t)B.n * B.g) return;
-    const int n = (int)(id / B.g), g = (int)(id % B.g);
-    const int len = valid_rows(B, n);
-    double s1 = 0.0, s2 = 0.0;
-    const int64_t items = (int64_t)B.chunks * B.d;
-    for (int64_t i = lane; i < items; i += 32) {
-        const int k = (int)(i / B.d), c = g * B.d + (int)(i % B.d);
-        const float2 v = part[((int64_t)n * B.chunks + k) * B.c + c];
-        const double w = B.w ? ld_param(B.w, B.ptype, c) : 1.0f;
-        s1 += w * v.x;
-        s2 += w * v.y;
-    }
-    for (int o = 16; o; o /= 2) {
-        s1 += __shfl_xor_sync(~0u, s1, o);
-        s2 += __shfl_xor_sync(~0u, s2, o);
-    }
-    const double count = len ? (double)len * B.d : 1.0;
-    if (lane == 0) means[id] = make_float2((float)(s1 / count), (float)(s2 / count));
-}
-
-// dbias and dweight: 32 channels per block, its warps taking the rows of part
-// in turn.
-__global__ void __launch_bounds__(kThreads)
-    k_back_params(const float2* __restrict__ part, int64_t rows, int c, float* __restrict__ dw,
-                  float* __restrict__ db) {
-    __shared__ double2 sm[kThreads / 32][32];
+// Adds `rows` rows of part for each of a number of spans, in double: to
+// tot[span][c], and to dbias and dweight where there is one span. A block takes
+// 32 channels of a span, its warps the rows in turn.
+constexpr int kAdd = 1024;
+__global__ void __launch_bounds__(kAdd)
+    k_back_join(const float2* __restrict__ part, int64_t rows, int c, int blocks,
+                float2* __restrict__ tot, float* __restrict__ dw, float* __restrict__ db) {
+    __shared__ double2 sm[kAdd / 32][33];
+    grid_wait();
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int ch = blockIdx.x * 32 + lane;
+    const int64_t span = blockIdx.x / blocks;
+    const int ch = blockIdx.x % blocks * 32 + lane;
+    const float2* p = part + span * rows * c + ch;
     double2 s = make_double2(0.0, 0.0);
-    if (ch < c)
-        for (int64_t r = warp; r < rows; r += kThreads / 32) {
-            const float2 v = part[r * c + ch];
+    if (ch < c) {
+#pragma unroll 4
+        for (int64_t r = warp; r < rows; r += kAdd / 32) {
+            const float2 v = p[r * c];
             s.x += v.x;
             s.y += v.y;
         }
+    }
     sm[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && ch < c) {
-        for (int w = 1; w < kThreads / 32; w++) {
-            s.x += sm[w][lane].x;
-            s.y += sm[w][lane].y;
+    for (int h = kAdd / 64; h; h /= 2) {
+        if (warp < h) {
+            sm[warp][lane].x += sm[warp + h][lane].x;
+            sm[warp][lane].y += sm[warp + h][lane].y;
         }
+        __syncthreads();
+    }
+    grid_release();
+    if (warp == 0 && ch < c) {
+        s = sm[0][lane];
+        if (tot) tot[span * c + ch] = make_float2((float)s.x, (float)s.y);
         if (db) db[ch] = (float)s.x;
         if (dw) dw[ch] = (float)s.y;
     }
 }
 
-template <class T, int AW, bool kFrom>
-__global__ void __launch_bounds__(kThreads)
-    k_back_apply(Batch B, const float2* __restrict__ means) {
-    constexpr int U = 2;
-    const int n = blockIdx.x / B.chunks;
+template <class T, int AW, bool kFrom, bool kSame>
+__global__ void __launch_bounds__(kThreads, 2)
+    k_back_apply(Batch B, const float2* __restrict__ tot) {
+    extern __shared__ float2 means[];  // of every group
+    grid_wait();
+    const int id = gridDim.x - 1 - blockIdx.x, n = id / B.chunks;
+    const int len = valid_rows(B, n);
     int r0, r1;
-    chunk_rows(valid_rows(B, n), B.chunks, blockIdx.x % B.chunks, r0, r1);
+    chunk_rows(len, B.chunks, id % B.chunks, r0, r1);
     if (r0 >= r1) return;
-    const T* dy = (const T*)B.dy + (int64_t)n * B.ys;
-    T* dx = (T*)B.out + (int64_t)n * B.os;
+    const float inv = 1.0f / ((float)len * (float)B.d);
+    group_sums(B, 0, B.g, [&](int i) { return __ldg(tot + (int64_t)n * B.c + i); },
+               [&](int g, float2 v) { means[g] = make_float2(v.x * inv, v.y * inv); });
+    __syncthreads();
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
     if (phase >= B.phases) return;
+    const PairStore<T, kFrom> none(nullptr, 0);
     for (int t = 0; t < B.tiles; t++) {
         const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
         if (unit >= B.units) break;
-        Params q;
-        load_params(B, n, unit, q);
-        float s1[8], s2[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int c = min(unit * kUnit + i, B.c - 1);
-            const float2 v = __ldg(means + (int64_t)n * B.g + c / B.d);
-            s1[i] = v.x;
-            s2[i] = v.y;
-        }
-        for (int r = r0 + phase; r < r1; r += U * B.phases) {
-            Raw<T> g[U];
-            Input<T, AW, kFrom> x[U];
-#pragma unroll
-            for (int j = 0; j < U; j++) {
-                const int rr = r + j * B.phases;
-                if (rr < r1) {
-                    g[j] = ld_unit<T, AW>(dy + (int64_t)rr * B.yr + unit * kUnit, cnt);
-                    x[j].load(B, n, rr, unit, cnt);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < U; j++) {
-                const int rr = r + j * B.phases;
-                if (rr < r1) {
-                    float xh[8], dz[8];
-                    x[j].get(xh);
-                    slopes(B, q, g[j], xh, dz);
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        dz[i] = q.rstd[i] * (__fmaf_rn(dz[i], q.w[i], -s1[i]) - xh[i] * s2[i]);
-                    Raw<T> o;
-                    pack(dz, o);
-                    st_unit<T, AW>(dx + (int64_t)rr * B.orow + unit * kUnit, o, cnt);
-                }
-            }
-        }
+        const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, true);
+        const int first = unit * kUnit;
+        const auto s1 = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return means[g].x; });
+        const auto s2 = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return means[g].y; });
+        back_rows<T, AW, kFrom, kSame>(B, q, s1, s2, n, r0, r1, phase, unit, cnt, none);
     }
 }
 
@@ -591,36 +953,153 @@ Region batch(const char* K, const char* name, const void* p, const simtgo_group_
     return r;
 }
 
-void fill(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool kept) {
+// Lets a kernel have as much shared memory as a block may, once per device.
+template <auto Kernel>
+int allow_smem(const sg::DevInfo& d, size_t bytes) {
+    static std::atomic<bool> done[64];
+    if (bytes <= 48 * 1024 || done[d.device & 63].load(std::memory_order_relaxed)) return 0;
+    cudaFuncAttributes at;
+    int rc = sg::cuda_status(cudaFuncGetAttributes(&at, Kernel), "cudaFuncGetAttributes(GroupNorm)");
+    if (!rc)
+        rc = sg::cuda_status(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                  d.max_smem_optin - (int)at.sharedSizeBytes),
+                             "cudaFuncSetAttribute(GroupNorm)");
+    if (!rc) done[d.device & 63].store(true, std::memory_order_relaxed);
+    return rc;
+}
+
+// Launches Kernel, as clusters of `cluster` blocks, and with `after` as soon as
+// the kernel before it releases it (it then waits for that one's end itself).
+template <auto Kernel, class... A>
+int launch(const sg::DevInfo& d, unsigned grid, int threads, size_t smem, cudaStream_t s,
+           int cluster, bool after, A... args) {
+    if (int rc = allow_smem<Kernel>(d, smem)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    cfg.attrs = at;
+    if (cluster > 1) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[cfg.numAttrs].val.clusterDim.x = cluster;
+        at[cfg.numAttrs].val.clusterDim.y = 1;
+        at[cfg.numAttrs].val.clusterDim.z = 1;
+        cfg.numAttrs++;
+    }
+    if (after) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs++;
+    }
+    sg::before_launch();
+    return sg::cuda_status(cudaLaunchKernelEx(&cfg, Kernel, args...), "GroupNorm");
+}
+
+// Tiles of at most 256 units for rows of `units`, whole blocks of `lanes`.
+void tile_units(Batch& B, int units, int lanes) {
+    const int upad = (units + lanes - 1) / lanes * lanes;
+    B.units = units;
+    B.tiles = (upad + kThreads - 1) / kThreads;
+    B.tile = ((upad + B.tiles - 1) / B.tiles + lanes - 1) / lanes * lanes;
+    B.tiles = (upad + B.tile - 1) / B.tile;
+    B.phases = kThreads / B.tile;
+}
+
+// How a call goes through its data. `elem` is the bytes of all inputs per
+// element; `sum_rows`, the rows a thread takes at a time; `iter_bytes`, what an
+// iteration of a block's threads keeps; `cell_bytes`, a thread's sums.
+struct Plan {
+    bool cluster;
+    unsigned grid;
+    size_t smem;
+};
+Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool keep_codes,
+               double elem, int sum_rows, int iter_bytes, int cell_bytes, int group_bytes) {
     B.n = c.samples;
     B.s = c.positions;
     B.c = c.channels;
     B.g = c.groups;
     B.d = c.channels / c.groups;
-    B.units = (c.channels + kUnit - 1) / kUnit;
-    B.lanes = kept ? std::min(c.block / kUnit, ceil_pow2(std::min(B.units, 32))) : 1;
-    B.shift = 0;
-    while (kept && (kUnit << B.shift) < c.block) B.shift++;
-    B.nblk = kept ? (c.channels + c.block - 1) / c.block : 0;
-    const int upad = (B.units + B.lanes - 1) / B.lanes * B.lanes;
-    B.tiles = (upad + kThreads - 1) / kThreads;
-    B.tile = ((upad + B.tiles - 1) / B.tiles + B.lanes - 1) / B.lanes * B.lanes;
-    B.tiles = (upad + B.tile - 1) / B.tile;
-    B.phases = kThreads / B.tile;
-    // Six blocks for each SM over the whole batch, but eight rows a thread.
-    const int64_t most = std::max<int64_t>(1, sg::ceil_div(B.s, 8 * B.phases));
-    B.chunks = (int)std::max<int64_t>(1, std::min(most, sg::ceil_div(6 * d.sms, B.n)));
     B.ptype = c.param_type;
     B.act = c.act;
     B.param = c.act_param;
     B.eps = c.eps;
+    const int units = (c.channels + kUnit - 1) / kUnit;
+
+    // A slab: whole groups, units and checkpoint blocks; 128 bytes of every row
+    // where the channels allow it, more while a slab would be a small load.
+    int64_t q = std::lcm((int64_t)B.d, (int64_t)kUnit);
+    if (keep_codes) q = std::lcm(q, (int64_t)c.block);
+    const int64_t most = kThreads * kUnit;
+    int64_t slab = c.channels;
+    if (q < c.channels) {
+        const int64_t least = 128 / elem_size(c.type);
+        slab = (least + q - 1) / q * q;
+        while (2 * slab <= std::min<int64_t>(c.channels, most) && slab * c.positions * elem < 65536)
+            slab *= 2;
+        slab = std::min<int64_t>(slab, c.channels);
+        const int64_t parts = (c.channels + slab - 1) / slab;
+        slab = std::min<int64_t>(((c.channels + parts - 1) / parts + q - 1) / q * q, c.channels);
+    }
+    Plan p = {};
+    if (slab <= most) {
+        const int slabs = (int)((c.channels + slab - 1) / slab);
+        const int su = (int)((slab + kUnit - 1) / kUnit);
+        const int lanes =
+            keep_codes ? std::min(c.block / kUnit, ceil_pow2(std::min(su, 32))) : 1;
+        Batch t = B;
+        tile_units(t, su, lanes);
+        t.slab = (int)slab;
+        t.slabs = slabs;
+        const int64_t clusters = (int64_t)c.samples * slabs;
+        const double bytes = (double)slab * c.positions * elem;
+        int k = 1;
+        while (k < 8 && c.positions / (2 * k) >= t.phases &&
+               (clusters * k < 2 * d.sms || bytes / k > 96 * 1024))
+            k *= 2;
+        t.chunks = k;
+        // A block moves about 36 GB/s; a chunked pass fills the GPU but costs
+        // two more launches, about 6 us.
+        const double us = bytes * clusters / (std::min<double>(clusters * k, 2 * d.sms) * 36e3);
+        const double chunked = bytes * clusters / 6.4e6 + 6.0;
+        if (us <= chunked && clusters * k <= 0x7fffffff) {
+            const size_t fixed = (size_t)t.phases * t.tile * cell_bytes +
+                                 (size_t)(slab / B.d + 1) * group_bytes + 32;
+            const size_t room = (clusters * k > d.sms ? (size_t)d.smem_per_sm / 2 : (size_t)d.max_smem_optin) - 4096;
+            const int64_t need = (c.positions / k + t.phases) / t.phases + 1;
+            int64_t keep = fixed < room ? (int64_t)(room - fixed) / iter_bytes : 0;
+            keep = std::min(keep, (need + sum_rows - 1) / sum_rows * sum_rows);
+            t.keep = (int)(keep / sum_rows * sum_rows);
+            p.smem = fixed + (size_t)t.keep * iter_bytes;
+            p.cluster = p.smem + 4096 <= (size_t)d.max_smem_optin;
+            p.grid = (unsigned)(clusters * k);
+            if (p.cluster) {
+                t.kept.lanes = lanes;
+                B = t;
+                return p;
+            }
+        }
+    }
+    const int lanes = keep_codes ? std::min(c.block / kUnit, ceil_pow2(std::min(units, 32))) : 1;
+    tile_units(B, units, lanes);
+    B.kept.lanes = lanes;
+    B.slab = c.channels;
+    B.slabs = 1;
+    B.keep = 0;
+    // One wave of blocks, eight rows a thread at least.
+    const int64_t rows = std::max<int64_t>(1, sg::ceil_div(B.s, 8 * B.phases));
+    B.chunks = (int)std::max<int64_t>(1, std::min(rows, (int64_t)3 * d.sms / std::max(1, B.n)));
+    p.grid = (unsigned)B.n * (unsigned)B.chunks;
+    return p;
 }
 
-template <class K>
-int allow_smem(K kernel, size_t bytes, const char* name) {
-    if (bytes <= 48 * 1024) return 0;
-    return sg::cuda_status(
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), name);
+void set_kept(Batch& B, const simtgo_group_norm& c, bool kept, int8_t* codes, float* scales) {
+    B.kept = {codes, scales, c.channels, 0, 0, 1};
+    if (!kept) return;
+    while ((kUnit << B.kept.shift) < c.block) B.kept.shift++;
+    B.kept.nblk = (c.channels + c.block - 1) / c.block;
 }
 
 }  // namespace
@@ -670,40 +1149,54 @@ int simtgo_GroupNorm(void* y, float* mean, float* rstd, const void* x, const voi
     B.w = weight;
     B.b = bias;
     B.lengths = lengths;
-    B.codes = codes;
-    B.scales = scales;
+    B.mean_out = mean;
+    B.rstd_out = rstd;
     B.xs = c.x_sample;
     B.xr = c.x_row;
     B.os = c.y_sample;
     B.orow = c.y_row;
-    fill(B, c, *d, kept);
-    int width = access_width(c.type, {{x, rx.pitch0 / elem_size(c.type), rx.pitch1 / elem_size(c.type)},
-                                      {y, ry.pitch0 / elem_size(c.type), ry.pitch1 / elem_size(c.type)}});
+    set_kept(B, c, kept, codes, scales);
+    const int e = elem_size(c.type);
+    int width = access_width(
+        c.type, {{x, rx.pitch0 / e, rx.pitch1 / e}, {y, ry.pitch0 / e, ry.pitch1 / e}});
     if (kept && width == 16 && (c.channels % kUnit || ((uintptr_t)codes & 7))) width = 4;
+    const bool same = (c.channels / c.groups) % kUnit == 0;
+    const Plan p = make_plan(B, c, *d, kept, e, e == 2 ? 8 : 4, kThreads * kUnit * e,
+                             (int)sizeof(Moments) * (same ? 1 : kUnit),
+                             (int)(sizeof(Moments) + sizeof(float2)));
     cudaStream_t s = (cudaStream_t)stream;
-    const int64_t parts = stats * B.chunks;
-    Scratch scratch;
-    if ((rc = scratch.alloc(sizeof(Moments) * parts + 8 * stats, s))) return rc;
-    Moments* part = (Moments*)scratch.p;
-    float* own = (float*)(part + parts);
-    float* mu = mean ? mean : own;
-    float* rs = rstd ? rstd : own + stats;
-    B.mean = mu;
-    B.rstd = rs;
-    const unsigned grid = (unsigned)B.chunks * (unsigned)B.n;
-    const size_t smem = sizeof(Moments) * kUnit * ((size_t)B.units + (size_t)B.phases * B.tile);
     return by_type(c.type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int AW = decltype(w)::value;
-        if (int e = allow_smem(k_stats<T, AW>, smem, K)) return e;
-        sg::before_launch();
-        k_stats<T, AW><<<grid, kThreads, smem, s>>>(B, part);
-        if (int e = sg::launch_status(K)) return e;
-        k_join<<<(unsigned)sg::ceil_div(stats, kThreads / 32), kThreads, 0, s>>>(B, part, mu, rs);
-        if (int e = sg::launch_status(K)) return e;
-        if (!elems) return 0;
-        k_apply<T, AW><<<grid, kThreads, 0, s>>>(B);
-        return sg::launch_status(K);
+        const auto run = [&](auto same_, auto kept_) -> int {
+            constexpr bool S = decltype(same_)::value, Q = decltype(kept_)::value;
+            if (p.cluster)
+                return launch<k_norm<T, AW, S, Q>>(*d, p.grid, kThreads, p.smem, s, B.chunks, false,
+                                                   B);
+            const int64_t parts = stats * B.chunks;
+            Scratch scratch;
+            if (int rc2 = scratch.alloc(sizeof(Moments) * parts + 8 * stats, s)) return rc2;
+            Moments* part = (Moments*)scratch.p;
+            float* own = (float*)(part + parts);
+            if (!mean) B.mean_out = own;
+            if (!rstd) B.rstd_out = own + stats;
+            const size_t smem =
+                sizeof(Moments) * (S ? 1 : kUnit) * ((size_t)B.units + (size_t)B.phases * B.tile);
+            if (int rc2 = launch<k_stats<T, AW, S>>(*d, p.grid, kThreads, smem, s, 1, false, B,
+                                                    part))
+                return rc2;
+            const int wide = std::min(32, ceil_pow2(c.groups));
+            const int blocks = (c.groups + wide - 1) / wide;
+            if (int rc2 = launch<k_join>(*d, (unsigned)c.samples * blocks, kJoin, 0, s, 1, true, B,
+                                         (const Moments*)part, wide, blocks))
+                return rc2;
+            if (!elems) return 0;
+            return launch<k_apply<T, AW, S, Q>>(*d, p.grid, kThreads, 0, s, 1, true, B);
+        };
+        if (same) return kept ? run(std::true_type(), std::true_type())
+                              : run(std::true_type(), std::false_type());
+        return kept ? run(std::false_type(), std::true_type())
+                    : run(std::false_type(), std::false_type());
     });
 }
 
@@ -782,42 +1275,68 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
     B.yr = c.y_row;
     B.os = c.d_sample;
     B.orow = c.d_row;
-    fill(B, c, *d, from);
+    set_kept(B, c, from, nullptr, nullptr);
     const int e = elem_size(c.type);
     int width = access_width(c.type, {{x, rx.pitch0 / e, rx.pitch1 / e},
                                       {dy, ry.pitch0 / e, ry.pitch1 / e},
                                       {dx, rd.pitch0 / e, rd.pitch1 / e}});
     if (from && width == 16 && (c.channels % kUnit || ((uintptr_t)codes & 7))) width = 4;
-    const int64_t parts = (int64_t)c.samples * B.chunks * c.channels;
+    const bool same = (c.channels / c.groups) % kUnit == 0;
+    const int unit_bytes = kUnit * e + (from ? 12 : kUnit * e);
+    const Plan p = make_plan(B, c, *d, false, from ? e + 1.1 : 2.0 * e, e == 2 ? 4 : 2,
+                             kThreads * unit_bytes, (int)sizeof(float2) * kUnit,
+                             2 * (int)sizeof(float2));
+    const bool params = dweight || dbias;
+    const int64_t parts = params || !p.cluster ? (int64_t)c.samples * B.chunks * c.channels : 0;
+    // A sample's own sums: the parts themselves where it is one chunk.
+    const bool spans = !p.cluster && dx && B.chunks > 1;
+    const int64_t tots = spans ? (int64_t)c.samples * c.channels : 0;
     Scratch scratch;
-    if ((rc = scratch.alloc(sizeof(float2) * (parts + stats), s))) return rc;
+    if (parts && (rc = scratch.alloc(sizeof(float2) * (parts + tots), s))) return rc;
     float2* part = (float2*)scratch.p;
-    float2* means = part + parts;
-    const unsigned grid = (unsigned)B.chunks * (unsigned)B.n;
-    const size_t smem = sizeof(float2) * kUnit * (size_t)B.phases * B.tile;
+    float2* tot = spans ? part + parts : part;
+    const unsigned add = (unsigned)sg::ceil_div(c.channels, 32);
+    if (spans && (int64_t)add * c.samples > 0x7fffffff)
+        return sg::fail(SIMTGO_ESIZE, "channels: %s: too many samples of so many channels", K);
     return by_type(c.type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int AW = decltype(w)::value;
-        sg::before_launch();
-        if (from)
-            k_back_stats<T, AW, true><<<grid, kThreads, smem, s>>>(B, part);
-        else
-            k_back_stats<T, AW, false><<<grid, kThreads, smem, s>>>(B, part);
-        if (int r = sg::launch_status(K)) return r;
-        if (dweight || dbias) {
-            k_back_params<<<(unsigned)sg::ceil_div(c.channels, 32), kThreads, 0, s>>>(
-                part, (int64_t)c.samples * B.chunks, c.channels, dweight, dbias);
-            if (int r = sg::launch_status(K)) return r;
-        }
-        if (!dx) return 0;
-        k_back_groups<<<(unsigned)sg::ceil_div(stats, kThreads / 32), kThreads, 0, s>>>(B, part,
-                                                                                      means);
-        if (int r = sg::launch_status(K)) return r;
-        if (from)
-            k_back_apply<T, AW, true><<<grid, kThreads, 0, s>>>(B, means);
-        else
-            k_back_apply<T, AW, false><<<grid, kThreads, 0, s>>>(B, means);
-        return sg::launch_status(K);
+        const auto run = [&](auto from_, auto same_) -> int {
+            constexpr bool F = decltype(from_)::value, S = decltype(same_)::value;
+            if (p.cluster) {
+                if (int r = launch<k_norm_back<T, AW, F, S>>(*d, p.grid, kThreads, p.smem, s,
+                                                             B.chunks, false, B, part))
+                    return r;
+            } else {
+                const size_t smem = sizeof(float2) * kUnit * (size_t)B.phases * B.tile;
+                if (int r = launch<k_back_stats<T, AW, F, S>>(*d, p.grid, kThreads, smem, s, 1,
+                                                              false, B, part))
+                    return r;
+            }
+            const int64_t all = (int64_t)c.samples * B.chunks;
+            if (spans) {
+                const bool one = c.samples == 1;
+                if (int r = launch<k_back_join>(*d, add * c.samples, kAdd, 0, s, 1, true,
+                                                (const float2*)part, (int64_t)B.chunks, c.channels,
+                                                (int)add, tot, one ? dweight : nullptr,
+                                                one ? dbias : nullptr))
+                    return r;
+            }
+            if (params && !(spans && c.samples == 1))
+                if (int r = launch<k_back_join>(*d, add, kAdd, 0, s, 1, true,
+                                                (const float2*)(spans ? tot : part),
+                                                spans ? (int64_t)c.samples : all, c.channels,
+                                                (int)add, (float2*)nullptr, dweight, dbias))
+                    return r;
+            if (p.cluster || !dx) return 0;
+            return launch<k_back_apply<T, AW, F, S>>(*d, p.grid, kThreads,
+                                                     sizeof(float2) * (size_t)c.groups, s, 1, true,
+                                                     B, (const float2*)tot);
+        };
+        if (from) return same ? run(std::true_type(), std::true_type())
+                              : run(std::true_type(), std::false_type());
+        return same ? run(std::false_type(), std::true_type())
+                    : run(std::false_type(), std::false_type());
     });
 }
 
