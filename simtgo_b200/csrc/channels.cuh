@@ -134,7 +134,8 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 neg2(float2 v) { return make_float2(-v.x, -v.y); }
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return add2(a, neg2(b)); }
+// a - b, rounded once.
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, both(-1.0f), a); }
 
 __device__ __forceinline__ V8 unpack(const Raw<float>& r) {
     V8 v;
@@ -508,23 +509,37 @@ struct Kept {
     int shift, lanes;    // log2(units per block); lanes that hold one block
 };
 
+// A thread's place in a checkpoint: its unit's codes and its block's scale in
+// the first of its rows, and how far on the next of its rows are.
+struct KeptAt {
+    int8_t* codes;
+    float* scale;
+    int64_t codes_step, scale_step;
+};
+__device__ __forceinline__ KeptAt kept_at(const Kept& k, int64_t row, int64_t step, int unit) {
+    return {k.codes + row * k.channels + unit * kUnit, k.scales + row * k.nblk + (unit >> k.shift),
+            step * k.channels, step * k.nblk};
+}
+
 // Writes the checkpoint of the units that a warp's lanes hold of U rows: unit
-// `unit` (cnt channels; only where unit_on) of rows row + u*step, where live[u].
-// Every lane of the warp calls it, with zeros where it has no unit; live is the
-// same for the lanes of a block. The two divisions of a block's scale are shared
-// out: lane u of each block's lanes makes row u's, where there are that many.
-template <class T, int AW, int U>
-__device__ __forceinline__ void keep_units(const Raw<T> (&raw)[U], const Kept& k, int64_t row,
-                                           int64_t step, const bool (&live)[U], int unit, int cnt,
+// `unit` (cnt channels; only where unit_on) of the thread's rows from `at` on,
+// where live[u]. Every lane of the warp calls it, with zeros where it has no
+// unit; live is the same for the lanes of a block. The two divisions of a
+// block's scale are shared out: lane u of each block's lanes makes row u's,
+// where there are that many.
+template <class T, int AW, int U, bool kFlat = false>
+__device__ __forceinline__ void keep_units(const Raw<T> (&raw)[U], const Kept& k, const KeptAt& at,
+                                           const bool (&live)[U], int unit, int cnt,
                                            bool unit_on) {
     uint32_t m[U];
     block_max<U>(raw, k.lanes, m);
     float inverse[U];
-    const int blk = unit >> k.shift;
+    const bool block_on = kFlat || (unit >> k.shift) < k.nblk;
     if (k.lanes >= U) {
         const int mine = threadIdx.x & (U - 1);
         uint32_t sel = m[0];
         bool sel_on = live[0];
+        float* to = at.scale;
 #pragma unroll
         for (int u = 1; u < U; u++) {
             sel = mine == u ? m[u] : sel;
@@ -535,22 +550,21 @@ __device__ __forceinline__ void keep_units(const Raw<T> (&raw)[U], const Kept& k
 #pragma unroll
         for (int u = 0; u < U; u++)
             inverse[u] = __shfl_sync(~0u, inv, (threadIdx.x & 31 & ~(U - 1)) + u);
-        if (sel_on && unit % k.lanes == mine && blk < k.nblk)
-            k.scales[(row + mine * step) * k.nblk + blk] = scale;
+        if (sel_on && (unit & (k.lanes - 1)) == mine && block_on) to[mine * at.scale_step] = scale;
     } else {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float scale;
             block_scale(m[u], scale, inverse[u]);
-            if (live[u] && unit % k.lanes == 0 && blk < k.nblk)
-                k.scales[(row + u * step) * k.nblk + blk] = scale;
+            if (live[u] && (unit & (k.lanes - 1)) == 0 && block_on)
+                at.scale[u * at.scale_step] = scale;
         }
     }
 #pragma unroll
     for (int u = 0; u < U; u++)
         if (unit_on && live[u])
-            st_codes<AW == 16>(k.codes + (row + u * step) * k.channels + unit * kUnit,
-                               encode(unpack(raw[u]), inverse[u]), cnt);
+            st_codes<AW == 16>(at.codes + u * at.codes_step, encode(unpack(raw[u]), inverse[u]),
+                               cnt);
 }
 
 // ---- host helpers -------------------------------------------------------------------

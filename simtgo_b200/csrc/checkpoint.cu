@@ -73,18 +73,25 @@ using namespace chan;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kIters = 8;  // units a thread takes at most
+template <class T>
+constexpr int kBackRows = sizeof(T) == 2 ? 4 : 2;
 constexpr int64_t kMaxElems = int64_t(1) << 46;  // keeps every byte offset far inside 64 bits
 
-// How rows of units fall on blocks: a tile of `tile` units by `phases` rows
-// at a time, `iters` times down the rows.
+// How units fall on blocks. Rows of units: a tile of `tile` units by `phases`
+// rows at a time, `iters` times down the rows. Where every matrix is contiguous
+// and its rows are whole checkpoint blocks (flat), rows mean nothing: a block
+// takes kThreads consecutive units, `iters` times, and no index needs a division
+// or a product.
 struct RowGrid {
-    int64_t rows;
+    int64_t rows, units_total;
     int channels, units, lanes, tiles, tile, phases, iters;
     int shift;  // log2(units per checkpoint block)
     int nblk;   // checkpoint blocks per row
+    bool flat;
 };
 
-RowGrid row_grid(int64_t rows, int channels, int block, int sms) {
+RowGrid row_grid(int64_t rows, int channels, int block, bool contiguous, int sms) {
     RowGrid g;
     g.rows = rows;
     g.channels = channels;
@@ -95,98 +102,142 @@ RowGrid row_grid(int64_t rows, int channels, int block, int sms) {
     g.shift = 0;
     while (block && (kUnit << g.shift) < block) g.shift++;
     g.nblk = block ? (channels + block - 1) / block : 0;
+    g.flat = contiguous && channels % (block ? block : kUnit) == 0;
+    g.units_total = g.flat ? rows * g.units : 0;
     const int upad = (g.units + g.lanes - 1) / g.lanes * g.lanes;
     g.tiles = (upad + kThreads - 1) / kThreads;
     g.tile = ((upad + g.tiles - 1) / g.tiles + g.lanes - 1) / g.lanes * g.lanes;
     g.tiles = (upad + g.tile - 1) / g.tile;
     g.phases = kThreads / g.tile;
-    // Eight rows a thread where there is work for many blocks, fewer when
+    // Eight units a thread where there is work for many blocks, fewer when
     // that would leave SMs idle.
-    const int64_t groups = sg::ceil_div(rows, g.phases) * g.tiles;
-    g.iters = (int)std::max<int64_t>(1, std::min<int64_t>(8, groups / (sms * 8)));
-    while (sg::ceil_div(rows, (int64_t)g.phases * g.iters) * g.tiles > 0x7fffffff) g.iters *= 2;
+    const int64_t groups =
+        g.flat ? sg::ceil_div(g.units_total, kThreads) : sg::ceil_div(rows, g.phases) * g.tiles;
+    g.iters = (int)std::max<int64_t>(1, std::min<int64_t>(kIters, groups / (sms * 8)));
+    while (groups / g.iters > 0x7ffffff0) g.iters *= 2;
     return g;
 }
 Kept kept(const RowGrid& g, int8_t* codes, float* scales) {
     return {codes, scales, g.channels, g.nblk, g.shift, g.lanes};
 }
 int64_t row_blocks(const RowGrid& g) {
+    if (g.flat) return sg::ceil_div(g.units_total, (int64_t)kThreads * g.iters);
     return sg::ceil_div(g.rows, (int64_t)g.phases * g.iters) * g.tiles;
 }
 
-// This thread's unit and first row. `on` is false for threads beyond the
-// tile's or the row's units; they still take part in shuffles.
+// This thread's unit, its first row and the number of its rows (phases apart);
+// `most` is the block's largest such number, over which every thread loops so
+// that shuffles find whole warps. `on` is false for threads beyond the tile's or
+// the row's units. Flat: `row` is the thread's first unit, and the next ones lie
+// kThreads units apart.
+template <bool kFlat>
 struct Place {
-    int64_t row0, end;  // block's first row and one past its last
-    int phase, unit, cnt;
+    int64_t row;
+    int rows, most, unit, cnt, phases;
     bool on;
+    __device__ __forceinline__ Place(const RowGrid& g) {
+        if (kFlat) {
+            const int64_t first = (int64_t)blockIdx.x * kThreads * g.iters;
+            const int64_t left = g.units_total - first;
+            most = (int)min((int64_t)g.iters, (left + kThreads - 1) / kThreads);
+            const int64_t mine = left - threadIdx.x;
+            rows = (int)min((int64_t)most, mine > 0 ? (mine + kThreads - 1) / kThreads : 0);
+            row = first + threadIdx.x;
+            unit = threadIdx.x & 31;  // a block's lanes are told by it
+            cnt = kUnit;
+            on = true;
+            return;
+        }
+        const int tile = blockIdx.x % g.tiles, phase = threadIdx.x / g.tile;
+        const int64_t row0 = (int64_t)(blockIdx.x / g.tiles) * g.phases * g.iters;
+        const int left = (int)min((int64_t)g.phases * g.iters, g.rows - row0);
+        row = row0 + phase;
+        most = (left + g.phases - 1) / g.phases;
+        rows = phase < g.phases ? (left - phase + g.phases - 1) / g.phases : 0;
+        unit = tile * g.tile + threadIdx.x % g.tile;
+        on = unit < g.units;
+        cnt = min(kUnit, g.channels - unit * kUnit);
+        phases = g.phases;
+    }
 };
-__device__ __forceinline__ Place place(const RowGrid& g) {
-    Place p;
-    const int tile = blockIdx.x % g.tiles;
-    p.row0 = (int64_t)(blockIdx.x / g.tiles) * g.phases * g.iters;
-    p.end = min(p.row0 + (int64_t)g.phases * g.iters, g.rows);
-    p.phase = threadIdx.x / g.tile;
-    p.unit = tile * g.tile + threadIdx.x % g.tile;
-    p.on = p.phase < g.phases && p.unit < g.units;
-    p.cnt = min(kUnit, g.channels - p.unit * kUnit);
-    return p;
-}
+// A thread's walk down one matrix: its unit in the first of its rows, and the
+// elements to the next.
+template <class T, bool kFlat>
+struct Walk {
+    T* at;
+    int64_t apart;
+    __device__ __forceinline__ Walk(T* base, int64_t pitch, const Place<kFlat>& p) {
+        at = base + (kFlat ? p.row * kUnit : p.row * pitch + p.unit * kUnit);
+        apart = kFlat ? 0 : p.phases * pitch;
+    }
+    __device__ __forceinline__ int64_t step() const { return kFlat ? kThreads * kUnit : apart; }
+    __device__ __forceinline__ T* ahead(int u) const { return at + u * step(); }
+    __device__ __forceinline__ void move(int u) { at += u * step(); }
+};
+// The same down a checkpoint.
+template <bool kFlat>
+struct KeptWalk {
+    KeptAt at;
+    __device__ __forceinline__ KeptWalk(const Kept& k, const Place<kFlat>& p) {
+        if (kFlat)
+            at = {k.codes + p.row * kUnit, k.scales + (p.row >> k.shift), kThreads * kUnit,
+                  kThreads >> k.shift};
+        else
+            at = kept_at(k, p.row, p.phases, p.unit);
+    }
+    __device__ __forceinline__ void move(int u) {
+        at.codes += u * (kFlat ? kThreads * kUnit : at.codes_step);
+        at.scale += u * at.scale_step;
+    }
+};
 
-// The rows of one step of a thread's loop: row0 + u*phases for u < U.
-template <int U>
-__device__ __forceinline__ void live_rows(const RowGrid& g, const Place& p, int64_t row,
-                                          bool (&live)[U]) {
-#pragma unroll
-    for (int u = 0; u < U; u++)
-        live[u] = p.phase < g.phases && row + (int64_t)u * g.phases < p.end;
-}
-
-template <class T, int AW>
+template <class T, int AW, bool kFlat>
 __global__ void __launch_bounds__(kThreads)
     k_pack8(Kept kept, const T* __restrict__ x, int64_t pitch, RowGrid g) {
     constexpr int U = 4;
-    const Place p = place(g);
-    const T* at = x + p.unit * kUnit;
-    for (int64_t row = p.row0 + p.phase; row - p.phase < p.end; row += (int64_t)U * g.phases) {
+    const Place<kFlat> p(g);
+    Walk<const T, kFlat> in(x, pitch, p);
+    KeptWalk<kFlat> out(kept, p);
+    for (int it = 0; it < p.most; it += U) {
         bool live[U];
-        live_rows<U>(g, p, row, live);
         Raw<T> raw[U] = {};
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (p.on && live[u])
-                raw[u] = ld_unit<T, AW>(at + (row + (int64_t)u * g.phases) * pitch, p.cnt);
-        keep_units<T, AW, U>(raw, kept, row, g.phases, live, p.unit, p.cnt, p.on);
+        for (int u = 0; u < U; u++) {
+            live[u] = it + u < p.rows;
+            if (p.on && live[u]) raw[u] = ld_unit<T, AW>(in.ahead(u), p.cnt);
+        }
+        keep_units<T, AW, U, kFlat>(raw, kept, out.at, live, p.unit, p.cnt, p.on);
+        in.move(U);
+        out.move(U);
     }
 }
 
-template <class T, int AW>
+template <class T, int AW, bool kFlat>
 __global__ void __launch_bounds__(kThreads)
-    k_unpack8(T* __restrict__ x, const int8_t* __restrict__ codes,
-              const float* __restrict__ scales, int64_t pitch, RowGrid g) {
+    k_unpack8(T* __restrict__ x, Kept kept, int64_t pitch, RowGrid g) {
     constexpr int U = 4;
-    const Place p = place(g);
+    const Place<kFlat> p(g);
     if (!p.on) return;
-    for (int64_t base = p.row0 + p.phase; base < p.end; base += (int64_t)U * g.phases) {
+    Walk<T, kFlat> out(x, pitch, p);
+    KeptWalk<kFlat> in(kept, p);
+    for (int it = 0; it < p.rows; it += U) {
         Codes c[U];
         float s[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t row = base + (int64_t)u * g.phases;
-            if (row < p.end) {
-                c[u] = ld_codes<AW == 16>(codes + row * g.channels + p.unit * kUnit, p.cnt);
-                s[u] = __ldg(scales + row * g.nblk + (p.unit >> g.shift));
+        for (int u = 0; u < U; u++)
+            if (it + u < p.rows) {
+                c[u] = ld_codes<AW == 16>(in.at.codes + u * in.at.codes_step, p.cnt);
+                s[u] = __ldg(in.at.scale + u * in.at.scale_step);
             }
-        }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t row = base + (int64_t)u * g.phases;
-            if (row < p.end) {
+        for (int u = 0; u < U; u++)
+            if (it + u < p.rows) {
                 Raw<T> r;
                 pack(decode(c[u], s[u]), r);
-                st_unit<T, AW>(x + row * pitch + p.unit * kUnit, r, p.cnt);
+                st_unit<T, AW>(out.ahead(u), r, p.cnt);
             }
-        }
+        in.move(U);
+        out.move(U);
     }
 }
 
@@ -201,24 +252,24 @@ struct GatedArgs {
     float param;
 };
 
-template <class T, int AW, bool kGate, bool kKeep>
+template <class T, int AW, bool kFlat, bool kGate, bool kKeep>
 __global__ void __launch_bounds__(kThreads) k_gated(GatedArgs k, RowGrid g) {
     constexpr int U = sizeof(T) == 2 ? 4 : 2;
-    const Place p = place(g);
-    const T* a = (const T*)k.a + p.unit * kUnit;
-    const T* b = (const T*)k.b + p.unit * kUnit;
-    T* y = (T*)k.y + p.unit * kUnit;
-    for (int64_t row = p.row0 + p.phase; row - p.phase < p.end; row += (int64_t)U * g.phases) {
+    const Place<kFlat> p(g);
+    Walk<const T, kFlat> a((const T*)k.a, k.a_pitch, p), b((const T*)k.b, k.b_pitch, p);
+    Walk<T, kFlat> y((T*)k.y, k.y_pitch, p);
+    KeptWalk<kFlat> ka(k.ka, p), kb(k.kb, p);
+    for (int it = 0; it < p.most; it += U) {
         bool live[U];
-        live_rows<U>(g, p, row, live);
         Raw<T> ra[U] = {}, rb[U] = {};
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int u = 0; u < U; u++) {
+            live[u] = it + u < p.rows;
             if (p.on && live[u]) {
-                const int64_t at = row + (int64_t)u * g.phases;
-                ra[u] = ld_unit<T, AW>(a + at * k.a_pitch, p.cnt);
-                if (kGate) rb[u] = ld_unit<T, AW>(b + at * k.b_pitch, p.cnt);
+                ra[u] = ld_unit<T, AW>(a.ahead(u), p.cnt);
+                if (kGate) rb[u] = ld_unit<T, AW>(b.ahead(u), p.cnt);
             }
+        }
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (p.on && live[u]) {
@@ -231,66 +282,85 @@ __global__ void __launch_bounds__(kThreads) k_gated(GatedArgs k, RowGrid g) {
                 }
                 Raw<T> r;
                 pack(v, r);
-                st_unit<T, AW>(y + (row + (int64_t)u * g.phases) * k.y_pitch, r, p.cnt);
+                st_unit<T, AW>(y.ahead(u), r, p.cnt);
             }
         if (kKeep) {
             if (k.ka.codes)
-                keep_units<T, AW, U>(ra, k.ka, row, g.phases, live, p.unit, p.cnt, p.on);
+                keep_units<T, AW, U, kFlat>(ra, k.ka, ka.at, live, p.unit, p.cnt, p.on);
             if (kGate && k.kb.codes)
-                keep_units<T, AW, U>(rb, k.kb, row, g.phases, live, p.unit, p.cnt, p.on);
+                keep_units<T, AW, U, kFlat>(rb, k.kb, kb.at, live, p.unit, p.cnt, p.on);
+            ka.move(U);
+            kb.move(U);
         }
+        a.move(U);
+        b.move(U);
+        y.move(U);
     }
 }
 
 struct GatedBackArgs {
     void *da, *db;
     const void *dy, *a, *b;
-    const int8_t *a_codes, *b_codes;
-    const float *a_scales, *b_scales;
+    Kept ka, kb;
     int64_t a_pitch, b_pitch, y_pitch, da_pitch, db_pitch;
     int act;
     float param;
 };
 
-// A unit of an input, from the tensor or from its checkpoint.
-template <class T, int AW, bool kFrom>
+// A thread's walk down one input: the tensor, or its checkpoint.
+template <class T, int AW, bool kFlat, bool kFrom>
 struct Source {
-    Raw<T> raw;
-    Codes codes;
-    float scale;
-    __device__ __forceinline__ void load(const T* x, const int8_t* c, const float* s, int64_t pitch,
-                                         const RowGrid& g, const Place& p, int64_t row) {
+    Walk<const T, kFlat> x;
+    KeptWalk<kFlat> kept;
+    __device__ __forceinline__ Source(const void* base, const Kept& k, int64_t pitch,
+                                      const Place<kFlat>& p)
+        : x((const T*)base, pitch, p), kept(k, p) {}
+    struct Unit {
+        Raw<T> raw;
+        Codes codes;
+        float scale;
+        __device__ __forceinline__ V8 get() const {
+            return kFrom ? decode(codes, scale) : unpack(raw);
+        }
+    };
+    __device__ __forceinline__ void load(Unit& v, int u, int cnt) const {
         if (kFrom) {
-            codes = ld_codes<AW == 16>(c + row * g.channels + p.unit * kUnit, p.cnt);
-            scale = __ldg(s + row * g.nblk + (p.unit >> g.shift));
+            v.codes = ld_codes<AW == 16>(kept.at.codes + u * kept.at.codes_step, cnt);
+            v.scale = __ldg(kept.at.scale + u * kept.at.scale_step);
         } else {
-            raw = ld_unit<T, AW>(x + row * pitch + p.unit * kUnit, p.cnt);
+            v.raw = ld_unit<T, AW>(x.ahead(u), cnt);
         }
     }
-    __device__ __forceinline__ V8 get() const { return kFrom ? decode(codes, scale) : unpack(raw); }
+    __device__ __forceinline__ void move(int u) {
+        if (kFrom)
+            kept.move(u);
+        else
+            x.move(u);
+    }
 };
 
-template <class T, int AW, bool kFrom, bool kGate>
+template <class T, int AW, bool kFlat, bool kFrom, bool kGate>
 __global__ void __launch_bounds__(kThreads) k_gated_back(GatedBackArgs k, RowGrid g) {
-    constexpr int U = sizeof(T) == 2 ? 4 : 2;
-    const Place p = place(g);
+    constexpr int U = kBackRows<T>;
+    const Place<kFlat> p(g);
     if (!p.on) return;
-    for (int64_t base = p.row0 + p.phase; base < p.end; base += (int64_t)U * g.phases) {
-        Source<T, AW, kFrom> a[U], b[U];
+    using In = Source<T, AW, kFlat, kFrom>;
+    In sa(k.a, k.ka, k.a_pitch, p), sb(k.b, k.kb, k.b_pitch, p);
+    Walk<const T, kFlat> y((const T*)k.dy, k.y_pitch, p);
+    Walk<T, kFlat> oa((T*)k.da, k.da_pitch, p), ob((T*)k.db, k.db_pitch, p);
+    for (int it = 0; it < p.rows; it += U) {
+        typename In::Unit a[U], b[U];
         Raw<T> dy[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t row = base + (int64_t)u * g.phases;
-            if (row < p.end) {
-                dy[u] = ld_unit<T, AW>((const T*)k.dy + row * k.y_pitch + p.unit * kUnit, p.cnt);
-                a[u].load((const T*)k.a, k.a_codes, k.a_scales, k.a_pitch, g, p, row);
-                if (kGate) b[u].load((const T*)k.b, k.b_codes, k.b_scales, k.b_pitch, g, p, row);
+        for (int u = 0; u < U; u++)
+            if (it + u < p.rows) {
+                dy[u] = ld_unit<T, AW>(y.ahead(u), p.cnt);
+                sa.load(a[u], u, p.cnt);
+                if (kGate) sb.load(b[u], u, p.cnt);
             }
-        }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t row = base + (int64_t)u * g.phases;
-            if (row < p.end) {
+        for (int u = 0; u < U; u++)
+            if (it + u < p.rows) {
                 V8 f, s;
                 activate_slope<sizeof(T) == 2>(a[u].get(), f, s, k.act, k.param);
                 const V8 d = unpack(dy[u]);
@@ -299,7 +369,7 @@ __global__ void __launch_bounds__(kThreads) k_gated_back(GatedBackArgs k, RowGri
 #pragma unroll
                     for (int i = 0; i < 4; i++) f.p[i] = mul2(f.p[i], d.p[i]);
                     pack(f, r);
-                    st_unit<T, AW>((T*)k.db + row * k.db_pitch + p.unit * kUnit, r, p.cnt);
+                    st_unit<T, AW>(ob.ahead(u), r, p.cnt);
                 }
                 if (k.da) {
                     V8 w = d;
@@ -311,10 +381,14 @@ __global__ void __launch_bounds__(kThreads) k_gated_back(GatedBackArgs k, RowGri
 #pragma unroll
                     for (int i = 0; i < 4; i++) s.p[i] = mul2(s.p[i], w.p[i]);
                     pack(s, r);
-                    st_unit<T, AW>((T*)k.da + row * k.da_pitch + p.unit * kUnit, r, p.cnt);
+                    st_unit<T, AW>(oa.ahead(u), r, p.cnt);
                 }
             }
-        }
+        y.move(U);
+        sa.move(U);
+        sb.move(U);
+        oa.move(U);
+        ob.move(U);
     }
 }
 
@@ -390,14 +464,15 @@ int simtgo_Pack8(int8_t* codes, float* scales, const void* x, int32_t type, int6
         return rc;
     const sg::DevInfo* d;
     if ((rc = sg::current_device(&d))) return rc;
-    const RowGrid g = row_grid(rows, channels, block, d->sms);
+    const RowGrid g = row_grid(rows, channels, block, rows == 1 || row_pitch == channels, d->sms);
     const int width =
         with_codes(access_width(type, {{x, rows > 1 ? row_pitch : 0, 0}}), channels, {codes});
     return by_type(type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
+        const auto kernel = g.flat ? k_pack8<T, decltype(w)::value, true>
+                                   : k_pack8<T, decltype(w)::value, false>;
         sg::before_launch();
-        k_pack8<T, decltype(w)::value>
-            <<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(
+        kernel<<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(
                 kept(g, codes, scales), (const T*)x, row_pitch, g);
         return sg::launch_status(K);
     });
@@ -420,15 +495,17 @@ int simtgo_Unpack8(void* x, const int8_t* codes, const float* scales, int32_t ty
         return rc;
     const sg::DevInfo* d;
     if ((rc = sg::current_device(&d))) return rc;
-    RowGrid g = row_grid(rows, channels, block, d->sms);
+    const RowGrid g = row_grid(rows, channels, block, rows == 1 || row_pitch == channels, d->sms);
     const int width =
         with_codes(access_width(type, {{x, rows > 1 ? row_pitch : 0, 0}}), channels, {codes});
     return by_type(type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
+        const auto kernel = g.flat ? k_unpack8<T, decltype(w)::value, true>
+                                   : k_unpack8<T, decltype(w)::value, false>;
         sg::before_launch();
-        k_unpack8<T, decltype(w)::value><<<(unsigned)row_blocks(g), kThreads, 0,
-                                           (cudaStream_t)stream>>>((T*)x, codes, scales, row_pitch,
-                                                                   g);
+        kernel<<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(
+                (T*)x, kept(g, const_cast<int8_t*>(codes), const_cast<float*>(scales)), row_pitch,
+                g);
         return sg::launch_status(K);
     });
 }
@@ -465,7 +542,9 @@ int simtgo_Gated(void* y, const void* a, const void* b, int8_t* a_codes, float* 
         return rc;
     const sg::DevInfo* d;
     if ((rc = sg::current_device(&d))) return rc;
-    const RowGrid g = row_grid(c.rows, c.channels, ka || kb ? c.block : 0, d->sms);
+    const bool solid_rows = c.rows == 1 || (c.a_pitch == c.channels && c.y_pitch == c.channels &&
+                                            (!b || c.b_pitch == c.channels));
+    const RowGrid g = row_grid(c.rows, c.channels, ka || kb ? c.block : 0, solid_rows, d->sms);
     const int m = c.rows > 1;
     int width = access_width(c.type, {{y, m * c.y_pitch, 0}, {a, m * c.a_pitch, 0},
                                       {b, m * c.b_pitch, 0}});
@@ -475,8 +554,12 @@ int simtgo_Gated(void* y, const void* a, const void* b, int8_t* a_codes, float* 
     return by_type(c.type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int AW = decltype(w)::value;
-        const auto kernel = b ? (ka || kb ? k_gated<T, AW, true, true> : k_gated<T, AW, true, false>)
-                              : (ka ? k_gated<T, AW, false, true> : k_gated<T, AW, false, false>);
+        const auto pick = [&](auto flat) {
+            constexpr bool F = decltype(flat)::value;
+            return b ? (ka || kb ? k_gated<T, AW, F, true, true> : k_gated<T, AW, F, true, false>)
+                     : (ka ? k_gated<T, AW, F, false, true> : k_gated<T, AW, F, false, false>);
+        };
+        const auto kernel = g.flat ? pick(std::true_type()) : pick(std::false_type());
         sg::before_launch();
         kernel<<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(k, g);
         return sg::launch_status(K);
@@ -523,21 +606,32 @@ int simtgo_Gated_backward(void* da, void* db, const void* dy, const void* a, con
         return rc;
     const sg::DevInfo* d;
     if ((rc = sg::current_device(&d))) return rc;
-    const RowGrid g = row_grid(c.rows, c.channels, from ? c.block : 0, d->sms);
+    const bool solid_rows =
+        c.rows == 1 || (c.y_pitch == c.channels && (!a || c.a_pitch == c.channels) &&
+                        (!b || c.b_pitch == c.channels) && (!da || c.da_pitch == c.channels) &&
+                        (!db || c.db_pitch == c.channels));
+    const RowGrid g = row_grid(c.rows, c.channels, from ? c.block : 0, solid_rows, d->sms);
     const int m = c.rows > 1;
     int width = access_width(c.type, {{dy, m * c.y_pitch, 0}, {a, m * c.a_pitch, 0},
                                       {b, m * c.b_pitch, 0}, {da, m * c.da_pitch, 0},
                                       {db, m * c.db_pitch, 0}});
     if (from) width = with_codes(width, c.channels, {a_codes, b_codes});
-    const GatedBackArgs k = {da, db, dy, a, b, a_codes, b_codes, a_scales, b_scales,
+    const GatedBackArgs k = {da, db, dy, a, b,
+                             kept(g, const_cast<int8_t*>(a_codes), const_cast<float*>(a_scales)),
+                             kept(g, const_cast<int8_t*>(b_codes), const_cast<float*>(b_scales)),
                              c.a_pitch, c.b_pitch, c.y_pitch, c.da_pitch, c.db_pitch,
                              c.act, c.act_param};
     return by_type(c.type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int AW = decltype(w)::value;
-        const auto kernel =
-            from ? (gate ? k_gated_back<T, AW, true, true> : k_gated_back<T, AW, true, false>)
-                 : (gate ? k_gated_back<T, AW, false, true> : k_gated_back<T, AW, false, false>);
+        const auto pick = [&](auto flat) {
+            constexpr bool F = decltype(flat)::value;
+            return from ? (gate ? k_gated_back<T, AW, F, true, true>
+                                : k_gated_back<T, AW, F, true, false>)
+                        : (gate ? k_gated_back<T, AW, F, false, true>
+                                : k_gated_back<T, AW, F, false, false>);
+        };
+        const auto kernel = g.flat ? pick(std::true_type()) : pick(std::false_type());
         sg::before_launch();
         kernel<<<(unsigned)row_blocks(g), kThreads, 0, (cudaStream_t)stream>>>(k, g);
         return sg::launch_status(K);

@@ -43,12 +43,10 @@ constexpr int64_t kMaxElems = int64_t(1) << 46;
 struct Batch {
     const void *x, *dy, *w, *b;
     void* out;  // y, or dx
-    const int8_t* codes_in;
-    const float* scales_in;
     const float *mean, *rstd;
     float *mean_out, *rstd_out;
     const int32_t* lengths;
-    Kept kept;
+    Kept kept;  // written forward, read backward
     int64_t xs, xr, ys, yr, os, orow;
     int n, s, c, g, d;
     int units, tile, tiles, phases;  // of a row, or of a slab's row
@@ -159,13 +157,17 @@ __device__ __forceinline__ int unit_moments(const T* x, int64_t pitch, int r, in
         return 0;
     }
     float2 k[P], s1[P] = {}, s2[P] = {};
-    int n = 0;
+    const int n = (r1 - r + step - 1) / step;
+    const T* at = x + (int64_t)r * pitch;
+    const int64_t next = step * pitch;
     bool first = true;
-    for (int it = 0; r < r1; r += U * step, it += U) {
+    for (int it = 0; it < n; it += U) {
         Raw<T> raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (r + u * step < r1) raw[u] = ld_unit<T, AW>(x + (int64_t)(r + u * step) * pitch, cnt);
+        for (int u = 0; u < U; u++) {
+            if (it + u < n) raw[u] = ld_unit<T, AW>(at, cnt);
+            at += next;
+        }
         if (first) {
             const V8 v = unpack(raw[0]);
 #pragma unroll
@@ -174,7 +176,7 @@ __device__ __forceinline__ int unit_moments(const T* x, int64_t pitch, int r, in
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (r + u * step < r1) {
+            if (it + u < n) {
                 keep(it + u, raw[u]);
                 const V8 v = unpack(raw[u]);
 #pragma unroll
@@ -183,7 +185,6 @@ __device__ __forceinline__ int unit_moments(const T* x, int64_t pitch, int r, in
                     s1[kSame ? 0 : i] = add2(s1[kSame ? 0 : i], dv);
                     s2[kSame ? 0 : i] = fma2(dv, dv, s2[kSame ? 0 : i]);
                 }
-                n++;
             }
     }
     if (kSame) {
@@ -260,17 +261,28 @@ struct PerGroup {
     float2 v[kSame ? 1 : 4];
     __device__ __forceinline__ float2 operator[](int i) const { return v[kSame ? 0 : i]; }
 };
-// f(group) for each of the unit's channels.
+// f(group) for each of the unit's channels, at most `last`: the unit's first
+// group by a division, the next ones by counting.
 template <bool kSame, class F>
 __device__ __forceinline__ PerGroup<kSame> per_group(int c0, int last, int d, F&& f) {
     PerGroup<kSame> r;
+    int g = c0 / d;
     if (kSame) {
-        r.v[0] = both(f(c0 / d));
-    } else {
-#pragma unroll
-        for (int i = 0; i < (kSame ? 1 : 4); i++)
-            r.v[i] = make_float2(f(min(c0 + 2 * i, last) / d), f(min(c0 + 2 * i + 1, last) / d));
+        r.v[0] = both(f(g));
+        return r;
     }
+    int in = c0 - g * d;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        v[i] = f(g);
+        if (c0 + i < last && ++in == d) {
+            in = 0;
+            g++;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < (kSame ? 1 : 4); i++) r.v[i] = make_float2(v[2 * i], v[2 * i + 1]);
     return r;
 }
 
@@ -284,27 +296,36 @@ __device__ __forceinline__ void apply_rows(const Batch& B, int n, int r0, int r1
                                            const V8& scale, const V8& bias,
                                            const Raw<T>* kept_rows) {
     constexpr int U = kOutRows<T>;
-    const T* x = (const T*)B.x + (int64_t)n * B.xs + unit * kUnit;
-    T* y = (T*)B.out + (int64_t)n * B.os + unit * kUnit;
-    const int iters = (r1 - r0 + B.phases - 1) / B.phases;
-    for (int it = (iters - 1) / U * U; it >= 0 && iters > 0; it -= U) {
-        const int row = r0 + phase + it * B.phases;
+    const int most = (r1 - r0 + B.phases - 1) / B.phases;
+    if (most <= 0) return;
+    const int rows = phase < B.phases ? (r1 - r0 - phase + B.phases - 1) / B.phases : 0;
+    int it = (most - 1) / U * U;
+    const int64_t row = r0 + phase + (int64_t)it * B.phases;
+    const T* x = (const T*)B.x + n * B.xs + row * B.xr + unit * kUnit;
+    T* y = (T*)B.out + n * B.os + row * B.orow + unit * kUnit;
+    const int64_t xstep = B.phases * B.xr, ystep = B.phases * B.orow;
+    KeptAt kept;
+    if (kKeep) kept = kept_at(B.kept, (int64_t)n * B.s + row, B.phases, unit);
+    for (; it >= 0; it -= U) {
         bool live[U];
         Raw<T> raw[U] = {};
 #pragma unroll
-        for (int u = 0; u < U; u++) live[u] = phase < B.phases && row + u * B.phases < r1;
+        for (int u = 0; u < U; u++) live[u] = it + u < rows;
         if (it + U <= B.keep) {
 #pragma unroll
             for (int u = 0; u < U; u++)
                 if (on && live[u]) raw[u] = kept_rows[(it + u) * kThreads + threadIdx.x];
         } else {
+            const T* at = x;
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (on && live[u])
-                    raw[u] = ld_unit<T, AW>(x + (int64_t)(row + u * B.phases) * B.xr, cnt);
+            for (int u = 0; u < U; u++) {
+                if (on && live[u]) raw[u] = ld_unit<T, AW>(at, cnt);
+                at += xstep;
+            }
         }
+        T* to = y;
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int u = 0; u < U; u++) {
             if (on && live[u]) {
                 V8 v = unpack(raw[u]);
 #pragma unroll
@@ -313,11 +334,17 @@ __device__ __forceinline__ void apply_rows(const Batch& B, int n, int r0, int r1
                 activate<sizeof(T) == 2>(v, B.act, B.param);
                 Raw<T> o;
                 pack(v, o);
-                st_unit<T, AW>(y + (int64_t)(row + u * B.phases) * B.orow, o, cnt);
+                st_unit<T, AW>(to, o, cnt);
             }
-        if (kKeep)
-            keep_units<T, AW, U>(raw, B.kept, (int64_t)n * B.s + row, B.phases, live, unit, cnt,
-                                 on);
+            to += ystep;
+        }
+        if (kKeep) {
+            keep_units<T, AW, U>(raw, B.kept, kept, live, unit, cnt, on);
+            kept.codes -= U * kept.codes_step;
+            kept.scale -= U * kept.scale_step;
+        }
+        x -= U * xstep;
+        y -= U * ystep;
     }
 }
 
@@ -518,19 +545,42 @@ struct Pair {
     Raw<T> dy, x;
     Codes codes;
     float scale;
-    __device__ __forceinline__ void load(const Batch& B, int n, int r, int unit, int cnt) {
-        dy = ld_unit<T, AW>((const T*)B.dy + (int64_t)n * B.ys + (int64_t)r * B.yr + unit * kUnit,
-                            cnt);
+    __device__ __forceinline__ V8 input() const { return kFrom ? decode(codes, scale) : unpack(x); }
+};
+// A thread's walk along its rows of both.
+template <class T, int AW, bool kFrom>
+struct PairWalk {
+    const T *dy, *x;
+    KeptAt kept;
+    int64_t dy_step, x_step;
+    __device__ __forceinline__ PairWalk(const Batch& B, int n, int64_t row, int unit) {
+        dy = (const T*)B.dy + n * B.ys + row * B.yr + unit * kUnit;
+        dy_step = B.phases * B.yr;
         if (kFrom) {
-            const int64_t row = (int64_t)n * B.s + r;
-            codes = ld_codes<AW == 16>(B.codes_in + row * B.c + unit * kUnit, cnt);
-            scale = __ldg(B.scales_in + row * B.kept.nblk + (unit >> B.kept.shift));
+            kept = kept_at(B.kept, (int64_t)n * B.s + row, B.phases, unit);
         } else {
-            x = ld_unit<T, AW>((const T*)B.x + (int64_t)n * B.xs + (int64_t)r * B.xr + unit * kUnit,
-                               cnt);
+            x = (const T*)B.x + n * B.xs + row * B.xr + unit * kUnit;
+            x_step = B.phases * B.xr;
         }
     }
-    __device__ __forceinline__ V8 input() const { return kFrom ? decode(codes, scale) : unpack(x); }
+    __device__ __forceinline__ void load(Pair<T, AW, kFrom>& v, int cnt) const {
+        v.dy = ld_unit<T, AW>(dy, cnt);
+        if (kFrom) {
+            v.codes = ld_codes<AW == 16>(kept.codes, cnt);
+            v.scale = __ldg(kept.scale);
+        } else {
+            v.x = ld_unit<T, AW>(x, cnt);
+        }
+    }
+    __device__ __forceinline__ void move(int rows) {
+        dy += rows * dy_step;
+        if (kFrom) {
+            kept.codes += rows * kept.codes_step;
+            kept.scale += rows * kept.scale_step;
+        } else {
+            x += rows * x_step;
+        }
+    }
 };
 // The same in shared memory: arrays of iterations by threads.
 template <class T, bool kFrom>
@@ -617,14 +667,18 @@ __device__ __forceinline__ void back_sums(const Batch& B, const BackParams<kSame
                                           int r1, int unit, int cnt, float2 (&a)[4], float2 (&c)[4],
                                           F&& keep) {
     constexpr int U = kOutRows<T>;
-    for (int it = 0; r < r1; r += U * B.phases, it += U) {
+    const int rows = (r1 - r + B.phases - 1) / B.phases;
+    PairWalk<T, AW, kFrom> walk(B, n, r, unit);
+    for (int it = 0; it < rows; it += U) {
         Pair<T, AW, kFrom> in[U];
 #pragma unroll
-        for (int j = 0; j < U; j++)
-            if (r + j * B.phases < r1) in[j].load(B, n, r + j * B.phases, unit, cnt);
+        for (int j = 0; j < U; j++) {
+            if (it + j < rows) walk.load(in[j], cnt);
+            walk.move(1);
+        }
 #pragma unroll
         for (int j = 0; j < U; j++)
-            if (r + j * B.phases < r1) {
+            if (it + j < rows) {
                 keep(it + j, in[j]);
                 V8 xh, dz;
                 slopes(B, q, in[j], xh, dz);
@@ -693,41 +747,54 @@ __device__ __forceinline__ void group_sums(const Batch& B, int c0, int groups, A
     }
 }
 
-// dx of rows [r0, r1) of this thread's unit, last rows first.
+// dx of rows [r0, r1) of this thread's unit, last rows first. s1 and s2 are the
+// negated means, added.
 template <class T, int AW, bool kFrom, bool kSame>
 __device__ __forceinline__ void back_rows(const Batch& B, const BackParams<kSame>& q,
                                           const PerGroup<kSame>& s1, const PerGroup<kSame>& s2,
                                           int n, int r0, int r1, int phase, int unit, int cnt,
                                           const PairStore<T, kFrom>& store) {
     constexpr int U = kOutRows<T>;
-    T* dx = (T*)B.out + (int64_t)n * B.os + unit * kUnit;
-    const int iters = (r1 - r0 - phase + B.phases - 1) / B.phases;
-    for (int it = (iters - 1) / U * U; it >= 0 && iters > 0; it -= U) {
-        const int row = r0 + phase + it * B.phases;
+    const int rows = (r1 - r0 - phase + B.phases - 1) / B.phases;
+    if (rows <= 0) return;
+    int it = (rows - 1) / U * U;
+    const int64_t row = r0 + phase + (int64_t)it * B.phases;
+    PairWalk<T, AW, kFrom> walk(B, n, row, unit);
+    T* dx = (T*)B.out + n * B.os + row * B.orow + unit * kUnit;
+    const int64_t step = B.phases * B.orow;
+    for (; it >= 0; it -= U) {
         Pair<T, AW, kFrom> in[U];
         if (it + U <= B.keep) {
 #pragma unroll
             for (int j = 0; j < U; j++)
-                if (row + j * B.phases < r1) store.get(it + j, in[j]);
+                if (it + j < rows) store.get(it + j, in[j]);
+            walk.move(-U);
         } else {
 #pragma unroll
-            for (int j = 0; j < U; j++)
-                if (row + j * B.phases < r1) in[j].load(B, n, row + j * B.phases, unit, cnt);
+            for (int j = 0; j < U; j++) {
+                if (it + j < rows) walk.load(in[j], cnt);
+                walk.move(1);
+            }
+            walk.move(-2 * U);
         }
+        T* to = dx;
 #pragma unroll
-        for (int j = 0; j < U; j++)
-            if (row + j * B.phases < r1) {
+        for (int j = 0; j < U; j++) {
+            if (it + j < rows) {
                 V8 xh, dz;
                 slopes(B, q, in[j], xh, dz);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float2 v = fma2(dz.p[i], q.w.p[i], neg2(s1[i]));
-                    dz.p[i] = mul2(q.rstd[i], fma2(neg2(xh.p[i]), s2[i], v));
+                    const float2 v = fma2(dz.p[i], q.w.p[i], s1[i]);
+                    dz.p[i] = mul2(q.rstd[i], fma2(xh.p[i], s2[i], v));
                 }
                 Raw<T> o;
                 pack(dz, o);
-                st_unit<T, AW>(dx + (int64_t)(row + j * B.phases) * B.orow, o, cnt);
+                st_unit<T, AW>(to, o, cnt);
             }
+            to += step;
+        }
+        dx -= U * step;
     }
 }
 
@@ -775,7 +842,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_norm_back(Batch B, float2* __re
             x += ld_cluster(&own[g].x, k);
             y += ld_cluster(&own[g].y, k);
         }
-        const float inv = len ? 1.0f / ((float)len * (float)B.d) : 0.0f;
+        const float inv = len ? -1.0f / ((float)len * (float)B.d) : 0.0f;
         means[g] = make_float2(x * inv, y * inv);
     }
     cluster_arrive();
@@ -867,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     int r0, r1;
     chunk_rows(len, B.chunks, id % B.chunks, r0, r1);
     if (r0 >= r1) return;
-    const float inv = 1.0f / ((float)len * (float)B.d);
+    const float inv = -1.0f / ((float)len * (float)B.d);
     group_sums(B, 0, B.g, [&](int i) { return __ldg(tot + (int64_t)n * B.c + i); },
                [&](int g, float2 v) { means[g] = make_float2(v.x * inv, v.y * inv); });
     __syncthreads();
@@ -1095,8 +1162,10 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
     return p;
 }
 
-void set_kept(Batch& B, const simtgo_group_norm& c, bool kept, int8_t* codes, float* scales) {
-    B.kept = {codes, scales, c.channels, 0, 0, 1};
+// The checkpoint that is written, or -- backward -- read.
+void set_kept(Batch& B, const simtgo_group_norm& c, bool kept, const int8_t* codes,
+              const float* scales) {
+    B.kept = {const_cast<int8_t*>(codes), const_cast<float*>(scales), c.channels, 0, 0, 1};
     if (!kept) return;
     while ((kUnit << B.kept.shift) < c.block) B.kept.shift++;
     B.kept.nblk = (c.channels + c.block - 1) / c.block;
@@ -1262,8 +1331,6 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
     B.x = x;
     B.dy = dy;
     B.out = dx;
-    B.codes_in = codes;
-    B.scales_in = scales;
     B.mean = mean;
     B.rstd = rstd;
     B.w = weight;
@@ -1275,7 +1342,7 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
     B.yr = c.y_row;
     B.os = c.d_sample;
     B.orow = c.d_row;
-    set_kept(B, c, from, nullptr, nullptr);
+    set_kept(B, c, from, codes, scales);
     const int e = elem_size(c.type);
     int width = access_width(c.type, {{x, rx.pitch0 / e, rx.pitch1 / e},
                                       {dy, ry.pitch0 / e, ry.pitch1 / e},
