@@ -37,7 +37,17 @@ using namespace chan;
 
 namespace {
 
+#ifndef KB
+#define KB 3
+#endif
+#ifndef BKB
+#define BKB 2
+#endif
+#ifndef KA
+#define KA 2
+#endif
 constexpr int kThreads = 256;
+constexpr int kBlocks = KB, kBackBlocks = BKB;  // per SM, at least
 constexpr int64_t kMaxElems = int64_t(1) << 46;
 
 struct Batch {
@@ -52,16 +62,11 @@ struct Batch {
     int units, tile, tiles, phases;  // of a row, or of a slab's row
     int slab, slabs;                 // channels of a cluster's slab, slabs of a sample
     int chunks;                      // blocks that share a sample's rows
-    int keep;                        // iterations whose rows stay in shared memory
+    int keep, ahead;                 // batches of rows that stay in shared memory; in flight
+    int keep_all;                    // every batch stays: there is no ring
     int ptype, act;
     float param, eps;
 };
-
-// Rows a thread loads before it uses any: while summing, and while finishing.
-template <class T>
-constexpr int kSumRows = sizeof(T) == 2 ? 8 : 4;
-template <class T>
-constexpr int kOutRows = sizeof(T) == 2 ? 4 : 2;
 
 __device__ __forceinline__ int valid_rows(const Batch& B, int n) {
     return B.lengths ? min(max(__ldg(B.lengths + n), 0), B.s) : B.s;
@@ -73,7 +78,14 @@ __device__ __forceinline__ void chunk_rows(int len, int chunks, int k, int& r0, 
     r1 = min(r0 + per, len);
 }
 
+// Rows of [r0, r1) that fall to a phase.
+__device__ __forceinline__ int phase_rows(const Batch& B, int r0, int r1, int phase) {
+    return phase < B.phases ? (r1 - r0 - phase + B.phases - 1) / B.phases : 0;
+}
+
 // ---- between blocks and grids --------------------------------------------------
+
+constexpr int kCluster = 8;  // blocks of a cluster, at most
 
 __device__ __forceinline__ void cluster_arrive() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -101,7 +113,277 @@ __device__ __forceinline__ void grid_release() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// ---- sums ---------------------------------------------------------------------
+// ---- rows through shared memory --------------------------------------------------
+// A thread copies its own rows' units to its own places in shared memory,
+// asynchronously and several batches ahead, and reads them back itself: the
+// loads in flight cost no registers, no barrier is needed, and a batch that
+// stays there is read again without leaving the SM. The first `keep` batches of
+// a thread's rows have places of their own; the others share a ring of `ahead`.
+
+__device__ __forceinline__ uint32_t shared_addr(const void* p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if (kBytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes)
+                     : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the newest `ahead` - 1 groups of this thread have arrived.
+__device__ __forceinline__ void copy_wait(int ahead) {
+    if (ahead == 8)
+        asm volatile("cp.async.wait_group 7;" ::: "memory");
+    else if (ahead == 4)
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (ahead == 2)
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+__device__ __forceinline__ void st_shared(uint32_t a, uint32_t v) {
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+
+constexpr int kPlane = 16 * kThreads;  // 16 bytes of every thread
+
+// Unit of cnt channels at p to this thread's 16 bytes (two planes for float32)
+// at dst; channels it lacks become zeros.
+template <class T, int AW>
+__device__ __forceinline__ void copy_unit(uint32_t dst, const T* p, int cnt) {
+    if (AW == 16 && cnt == kUnit) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++)
+            copy_async<16>(dst + i * kPlane, reinterpret_cast<const char*>(p) + 16 * i);
+    } else if (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t to = dst + i / 4 * kPlane + i % 4 * 4;
+            if (i < cnt)
+                copy_async<4>(to, p + i);
+            else
+                st_shared(to, 0);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (2 * i + 1 < cnt)
+                copy_async<4>(dst + 4 * i, p + 2 * i);
+            else
+                st_shared(dst + 4 * i, 2 * i < cnt ? (uint32_t)*reinterpret_cast<const uint16_t*>(
+                                                         p + 2 * i)
+                                                   : 0u);
+        }
+    }
+}
+template <class T>
+__device__ __forceinline__ void store_unit(uint32_t dst, const Raw<T>& r) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + i * kPlane),
+                     "r"(r.q[i].x), "r"(r.q[i].y), "r"(r.q[i].z), "r"(r.q[i].w)
+                     : "memory");
+}
+template <class T>
+__device__ __forceinline__ Raw<T> shared_unit(uint32_t src) {
+    Raw<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.q[i].x), "=r"(r.q[i].y), "=r"(r.q[i].z), "=r"(r.q[i].w)
+                     : "r"(src + i * kPlane));
+    return r;
+}
+
+// What a row gives a thread: forward a unit of x; backward one of dy and one of
+// x, or of its checkpoint.
+template <class T>
+struct FwdRow {
+    static constexpr int kBytes = (int)sizeof(Raw<T>);
+    static constexpr int kRows = sizeof(T) == 2 ? 4 : 2;  // of a batch
+    const T* x;
+    int64_t step;
+    __device__ __forceinline__ FwdRow(const Batch& B, int n, int64_t row, int unit)
+        : x((const T*)B.x + n * B.xs + row * B.xr + unit * kUnit), step(B.phases * B.xr) {}
+    __device__ __forceinline__ void move(int rows) { x += rows * step; }
+    // The next U rows (where live) to consecutive slots; at ends past them.
+    template <int AW>
+    __device__ __forceinline__ void copy(uint32_t slot, int live, int cnt) {
+        constexpr int U = kRows;
+        if constexpr (AW == 2) {
+            Raw<T> r[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (u < live) r[u] = ld_unit<T, AW>(x, cnt);
+                x += step;
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (u < live) store_unit<T>(slot + u * kBytes * kThreads, r[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (u < live) copy_unit<T, AW>(slot + u * kBytes * kThreads, x, cnt);
+                x += step;
+            }
+        }
+    }
+};
+template <class T, bool kFrom>
+struct BackRow {
+    static constexpr int kX = (int)sizeof(Raw<T>) * kThreads;  // dy first
+    static constexpr int kBytes = (int)sizeof(Raw<T>) + (kFrom ? 12 : (int)sizeof(Raw<T>));
+    static constexpr int kRows = sizeof(T) == 2 ? 2 : 1;
+    const T *dy, *x;
+    const int8_t* codes;
+    const float* scale;
+    int64_t dy_step, x_step, scale_step;
+    __device__ __forceinline__ BackRow(const Batch& B, int n, int64_t row, int unit) {
+        dy = (const T*)B.dy + n * B.ys + row * B.yr + unit * kUnit;
+        dy_step = B.phases * B.yr;
+        if (kFrom) {
+            const KeptAt at = kept_at(B.kept, (int64_t)n * B.s + row, B.phases, unit);
+            codes = at.codes;
+            scale = at.scale;
+            x_step = at.codes_step;
+            scale_step = at.scale_step;
+        } else {
+            x = (const T*)B.x + n * B.xs + row * B.xr + unit * kUnit;
+            x_step = B.phases * B.xr;
+        }
+    }
+    __device__ __forceinline__ void move(int rows) {
+        dy += rows * dy_step;
+        if (kFrom) {
+            codes += rows * x_step;
+            scale += rows * scale_step;
+        } else {
+            x += rows * x_step;
+        }
+    }
+    template <int AW>
+    __device__ __forceinline__ void copy(uint32_t slot, int live, int cnt) {
+        constexpr int U = kRows;
+        const uint32_t cs = kX + threadIdx.x * 8 - threadIdx.x * 16;        // codes' place
+        const uint32_t ss = kX + 8 * kThreads + threadIdx.x * 4 - threadIdx.x * 16;
+        if constexpr (AW == 16) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint32_t to = slot + u * kBytes * kThreads;
+                if (u < live) {
+                    copy_unit<T, AW>(to, dy, cnt);
+                    if (kFrom) {
+                        copy_async<8>(to + cs, codes);
+                        copy_async<4>(to + ss, scale);
+                    } else {
+                        copy_unit<T, AW>(to + kX, x, cnt);
+                    }
+                }
+                move(1);
+            }
+        } else {
+            Raw<T> a[U], b[U];
+            Codes c[U];
+            float f[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (u < live) {
+                    a[u] = ld_unit<T, AW>(dy, cnt);
+                    if (kFrom) {
+                        c[u] = ld_codes<false>(codes, cnt);
+                        f[u] = __ldg(scale);
+                    } else {
+                        b[u] = ld_unit<T, AW>(x, cnt);
+                    }
+                }
+                move(1);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint32_t to = slot + u * kBytes * kThreads;
+                if (u < live) {
+                    store_unit<T>(to, a[u]);
+                    if (kFrom) {
+                        st_shared(to + cs, c[u].q.x);
+                        st_shared(to + cs + 4, c[u].q.y);
+                        st_shared(to + ss, __float_as_uint(f[u]));
+                    } else {
+                        store_unit<T>(to + kX, b[u]);
+                    }
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ V8 input(uint32_t slot) {
+        if (!kFrom) return unpack(shared_unit<T>(slot + kX));
+        Codes c;
+        float f;
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                     : "=r"(c.q.x), "=r"(c.q.y)
+                     : "r"(slot + kX + threadIdx.x * 8 - threadIdx.x * 16));
+        asm volatile("ld.shared.f32 %0, [%1];"
+                     : "=f"(f)
+                     : "r"(slot + kX + 8 * kThreads + threadIdx.x * 4 - threadIdx.x * 16));
+        return decode(c, f);
+    }
+};
+
+// A thread's rows in batches: `most` rows for the block's busiest thread, `mine`
+// for this one.
+template <class Row>
+struct Feed {
+    uint32_t base;
+    int keep, ahead, batches, mine;
+    __device__ __forceinline__ Feed(const Batch& B, void* smem, int most, int rows)
+        : base(shared_addr(smem) + threadIdx.x * 16),
+          keep(B.keep),
+          ahead(B.ahead),
+          batches((most + Row::kRows - 1) / Row::kRows),
+          mine(rows) {}
+    __device__ __forceinline__ uint32_t slot(int b) const {
+        const int at = b < keep ? b : keep + (b & (ahead - 1));
+        return base + at * (Row::kRows * Row::kBytes * kThreads);
+    }
+    // Batch by batch, first to last: f(slot, first row of the batch).
+    template <int AW, class F>
+    __device__ __forceinline__ void forward(Row row, int cnt, F&& f) const {
+        for (int b = 0; b < ahead; b++) {
+            if (b < batches) row.template copy<AW>(slot(b), mine - b * Row::kRows, cnt);
+            copy_commit();
+        }
+        for (int b = 0; b < batches; b++) {
+            copy_wait(ahead);
+            f(slot(b), b * Row::kRows);
+            if (b + ahead < batches)
+                row.template copy<AW>(slot(b + ahead), mine - (b + ahead) * Row::kRows, cnt);
+            copy_commit();
+        }
+    }
+    // Last to first; the kept batches are not copied again. `row` is the first.
+    template <int AW, class F>
+    __device__ __forceinline__ void backward(Row row, int cnt, F&& f) const {
+        int next = batches - 1;
+        row.move(next * Row::kRows);
+        const auto copy_next = [&]() {
+            if (next >= keep) {
+                row.template copy<AW>(slot(next), mine - next * Row::kRows, cnt);
+                row.move(-2 * Row::kRows);
+                next--;
+            }
+            copy_commit();
+        };
+        for (int j = 0; j < ahead; j++) copy_next();
+        for (int b = batches - 1; b >= 0; b--) {
+            if (b >= keep) copy_wait(ahead);
+            f(slot(b), b * Row::kRows);
+            if (b >= keep) copy_next();
+        }
+    }
+};
+
+// ---- moments ------------------------------------------------------------------
 // A cell is what a thread sums together: a channel, or -- where groups are whole
 // units (kSame) -- a unit.
 
@@ -113,72 +395,40 @@ struct Moments {  // the mean is k + off; m2: the sum of squared deviations from
 __device__ __forceinline__ Moments join(float na, Moments a, float nb, Moments b) {
     if (na == 0.0f) return b;
     const float f = nb / (na + nb), d = nb > 0.0f ? (b.k - a.k) + (b.off - a.off) : 0.0f;
-    return {a.k, __fmaf_rn(d, f, a.off), __fmaf_rn(d * d, na * f, a.m2 + b.m2)};
+    return {a.k, __fmaf_rn(d, f, a.off), __fmaf_rn(d * d, na * f, nb > 0.0f ? a.m2 + b.m2 : a.m2)};
 }
 
-// Joins the phases of a block's threads: red holds phase p's moments of
-// cell i at [p*width + i], cnt[p] its count. Phase 0 ends with them all. Every
-// thread calls it, after a barrier.
-template <int E>
-__device__ void join_phases(Moments* red, float* cnt, int phases, int width, int phase, int cell) {
-    float* in = cnt;
-    float* out = cnt + kThreads;
-    for (int m = phases; m > 1;) {
-        const int h = (m + 1) / 2;
-        if (phase < h) {
-            const bool two = phase + h < m;
-            const float na = in[phase], nb = two ? in[phase + h] : 0.0f;
-            if (two) {
-#pragma unroll
-                for (int i = 0; i < E; i++) {
-                    Moments* a = red + phase * width + cell + i;
-                    *a = join(na, *a, nb, a[h * width]);
-                }
-            }
-            if (cell == 0) out[phase] = na + nb;
-        }
-        float* t = in;
-        in = out;
-        out = t;
-        m = h;
-        __syncthreads();
+// The cells' moments of every phase in shared memory, arrays apart.
+struct CellSums {
+    float *k, *off, *m2;
+    int width;  // cells of a phase, padded so that phases start in other banks
+    __device__ __forceinline__ CellSums(float* base, int phases, int cells, bool units)
+        : width(units ? cells | 1 : cells + 4) {
+        k = base;
+        off = k + phases * width;
+        m2 = off + phases * width;
     }
+};
+__host__ __device__ constexpr int cell_floats(int phases, int cells, bool units) {
+    return 3 * phases * (units ? cells | 1 : cells + 4);
 }
 
-// Moments of this thread's cells over rows r0 + phase, + phases, ... < r1;
-// keep(it, raw) is handed every row's unit. Returns the number of rows.
-template <class T, int AW, bool kSame, class F>
-__device__ __forceinline__ int unit_moments(const T* x, int64_t pitch, int r, int r1, int step,
-                                            int cnt, Moments (&out)[kSame ? 1 : 8], F&& keep) {
-    constexpr int U = kSumRows<T>, P = kSame ? 1 : 4;
-    if (r >= r1) {
-#pragma unroll
-        for (int i = 0; i < (kSame ? 1 : 8); i++) out[i] = {0.0f, 0.0f, 0.0f};
-        return 0;
-    }
-    float2 k[P], s1[P] = {}, s2[P] = {};
-    const int n = (r1 - r + step - 1) / step;
-    const T* at = x + (int64_t)r * pitch;
-    const int64_t next = step * pitch;
-    bool first = true;
-    for (int it = 0; it < n; it += U) {
-        Raw<T> raw[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (it + u < n) raw[u] = ld_unit<T, AW>(at, cnt);
-            at += next;
-        }
-        if (first) {
-            const V8 v = unpack(raw[0]);
+// Sums this thread's cells down its rows and stores their moments.
+template <class T, int AW, bool kSame>
+__device__ __forceinline__ void sum_rows(const Feed<FwdRow<T>>& feed, const FwdRow<T>& rows,
+                                         int cnt, const CellSums& out, int phase, int u) {
+    constexpr int U = FwdRow<T>::kRows, P = kSame ? 1 : 4;
+    float2 k[P] = {}, s1[P] = {}, s2[P] = {};
+    feed.template forward<AW>(rows, cnt, [&](uint32_t slot, int first) {
+        if (first == 0 && feed.mine > 0) {
+            const V8 v = unpack(shared_unit<T>(slot));
 #pragma unroll
             for (int i = 0; i < P; i++) k[i] = kSame ? both(v.p[0].x) : v.p[i];
-            first = false;
         }
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (it + u < n) {
-                keep(it + u, raw[u]);
-                const V8 v = unpack(raw[u]);
+        for (int j = 0; j < U; j++)
+            if (first + j < feed.mine) {
+                const V8 v = unpack(shared_unit<T>(slot + j * FwdRow<T>::kBytes * kThreads));
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float2 dv = sub2(v.p[i], k[kSame ? 0 : i]);
@@ -186,48 +436,76 @@ __device__ __forceinline__ int unit_moments(const T* x, int64_t pitch, int r, in
                     s2[kSame ? 0 : i] = fma2(dv, dv, s2[kSame ? 0 : i]);
                 }
             }
-    }
-    if (kSame) {
-        const float a = s1[0].x + s1[0].y, q = s2[0].x + s2[0].y, m = a / (float)(8 * n);
+    });
+    const int at = phase * out.width + u * (kSame ? 1 : 8);
+    if constexpr (kSame) {
+        const float a = s1[0].x + s1[0].y, q = s2[0].x + s2[0].y;
+        const float m = feed.mine > 0 ? a / (float)(kUnit * feed.mine) : 0.0f;
         const float m2 = __fmaf_rn(-m, a, q);
-        out[0] = {k[0].x, m, m2 < 0.0f ? 0.0f : m2};
+        out.k[at] = k[0].x;
+        out.off[at] = m;
+        out.m2[at] = m2 < 0.0f ? 0.0f : m2;
     } else {
-        const float inv = 1.0f / (float)n;
+        const float2 inv = both(feed.mine > 0 ? 1.0f / (float)feed.mine : 0.0f);
+        float2 m[4], q[4];
 #pragma unroll
-        for (int i = 0; i < (kSame ? 1 : 8); i++) {
-            const float2 a = s1[i / 2 % P], q = s2[i / 2 % P], kk = k[i / 2 % P];
-            const float m = (i & 1 ? a.y : a.x) * inv;
-            const float m2 = __fmaf_rn(-m, i & 1 ? a.y : a.x, i & 1 ? q.y : q.x);
-            out[i] = {i & 1 ? kk.y : kk.x, m, m2 < 0.0f ? 0.0f : m2};
+        for (int i = 0; i < 4; i++) {
+            m[i] = mul2(s1[i], inv);
+            q[i] = fma2(neg2(m[i]), s1[i], s2[i]);
+            q[i] = make_float2(q[i].x < 0.0f ? 0.0f : q[i].x, q[i].y < 0.0f ? 0.0f : q[i].y);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const auto put = [&](float* to, float2 a, float2 b) {
+                *reinterpret_cast<float4*>(to + at + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
+            };
+            put(out.k, k[2 * i], k[2 * i + 1]);
+            put(out.off, m[2 * i], m[2 * i + 1]);
+            put(out.m2, q[2 * i], q[2 * i + 1]);
         }
     }
-    return n;
 }
 
-// Group moments from the moments of `d` cells each of `count` values: sub-warps
-// take a group each; f(group, moments) on the sub-warp's first lane.
+// Joins the cells [t0, t1) that lie in `sums` over all phases into the moments
+// of the groups of d cells they belong to, a cell's row holding `per` values:
+// f(group, count, moments) on one lane, for the part of the group inside. Rows
+// are dealt to the phases in turn. A sub-warp takes a group: two passes, the
+// mean of the cells' means about the first one, then the squares about it.
 template <class F>
-__device__ __forceinline__ void group_moments(const Moments* cells, int groups, int d, float count,
-                                              F&& f) {
-    int lanes = 1;
-    while (lanes < d && lanes < 32) lanes *= 2;
-    const int per = kThreads / lanes, lane = threadIdx.x % lanes;
-    for (int g0 = 0; g0 < groups; g0 += per) {
-        const int g = g0 + threadIdx.x / lanes;
-        const Moments* c = cells + (int64_t)g * d;
-        const float k = g < groups ? c[0].k : 0.0f;
-        float off = 0.0f, m2 = 0.0f;
-        if (g < groups)
-            for (int i = lane; i < d; i += lanes) off += (c[i].k - k) + c[i].off;
-        for (int o = lanes / 2; o; o /= 2) off += __shfl_xor_sync(~0u, off, o);
-        off /= (float)d;
-        if (g < groups)
-            for (int i = lane; i < d; i += lanes) {
-                const float dv = (c[i].k - k) + (c[i].off - off);
-                m2 += __fmaf_rn(count * dv, dv, c[i].m2);
-            }
-        for (int o = lanes / 2; o; o /= 2) m2 += __shfl_xor_sync(~0u, m2, o);
-        if (g < groups && lane == 0) f(g, Moments{k, off, m2});
+__device__ __forceinline__ void join_groups(const CellSums& sums, int phases, int rows, int t0,
+                                            int t1, int d, int per, F&& f) {
+    const int g_lo = t0 / d, groups = (t1 - 1) / d - g_lo + 1;
+    int along = 1;  // lanes along a group's cells; the others share out the phases
+    while (along < d && along < 32) along *= 2;
+    int lanes = 32;
+    while (lanes > along && groups * lanes > kThreads) lanes /= 2;
+    const int lane = threadIdx.x % lanes, lc = lane % along, lp = lane / along;
+    const int skip = lanes / along;
+    for (int base = 0; base < groups; base += kThreads / lanes) {
+        const int i = base + threadIdx.x / lanes, g = g_lo + i;
+        const bool on = i < groups;
+        const int c0 = on ? max(g * d, t0) - t0 : 0, c1 = on ? min(g * d + d, t1) - t0 : 0;
+        const float k0 = on ? sums.k[c0] : 0.0f, total = (float)rows * (float)(c1 - c0);
+        float a = 0.0f, q = 0.0f;
+        for (int p = lp; p < phases; p += skip) {
+            const float n = (float)max((rows - p + phases - 1) / phases, 0);
+            const int at = p * sums.width;
+            for (int c = c0 + lc; c < c1; c += along)
+                a = __fmaf_rn(n, n > 0.0f ? (sums.k[at + c] - k0) + sums.off[at + c] : 0.0f, a);
+        }
+        for (int o = lanes / 2; o; o /= 2) a += __shfl_xor_sync(~0u, a, o);
+        const float off = total > 0.0f ? a / total : 0.0f;
+        for (int p = lp; p < phases; p += skip) {
+            const float n = (float)max((rows - p + phases - 1) / phases, 0);
+            const int at = p * sums.width;
+            for (int c = c0 + lc; c < c1; c += along)
+                if (n > 0.0f) {
+                    const float dv = (sums.k[at + c] - k0) + (sums.off[at + c] - off);
+                    q += __fmaf_rn(n * (float)per * dv, dv, sums.m2[at + c]);
+                }
+        }
+        for (int o = lanes / 2; o; o /= 2) q += __shfl_xor_sync(~0u, q, o);
+        if (on && lane == 0) f(g, total * (float)per, Moments{k0, off, q});
     }
 }
 
@@ -267,70 +545,78 @@ template <bool kSame, class F>
 __device__ __forceinline__ PerGroup<kSame> per_group(int c0, int last, int d, F&& f) {
     PerGroup<kSame> r;
     int g = c0 / d;
-    if (kSame) {
+    if constexpr (kSame) {
         r.v[0] = both(f(g));
-        return r;
-    }
-    int in = c0 - g * d;
-    float v[8];
+    } else {
+        int in = c0 - g * d;
+        float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        v[i] = f(g);
-        if (c0 + i < last && ++in == d) {
-            in = 0;
-            g++;
+        for (int i = 0; i < 8; i++) {
+            v[i] = f(g);
+            if (c0 + i < last && ++in == d) {
+                in = 0;
+                g++;
+            }
         }
-    }
 #pragma unroll
-    for (int i = 0; i < (kSame ? 1 : 4); i++) r.v[i] = make_float2(v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < 4; i++) r.v[i] = make_float2(v[2 * i], v[2 * i + 1]);
+    }
     return r;
 }
 
 // ---- finishing rows, forward -----------------------------------------------------------
 
-// y (and the checkpoint) of rows [r0, r1) of this thread's unit, last rows
-// first; rows of iterations below B.keep come from `kept_rows`.
+struct Stat {
+    float mean, rstd;
+};
+// z = (x - mean)*scale + bias: the deviation first, so that it is exact where
+// the group hardly varies. The mean is held negated.
+template <bool kSame>
+struct Affine {
+    PerGroup<kSame> minus;
+    V8 scale, bias;
+};
+template <bool kSame, class F>
+__device__ __forceinline__ Affine<kSame> affine(const Batch& B, const V8& w, const V8& b, int first,
+                                                int last, F&& stat) {
+    Affine<kSame> a;
+    a.minus = per_group<kSame>(first, last, B.d, [&](int g) { return -stat(g).mean; });
+    const auto rstd = per_group<kSame>(first, last, B.d, [&](int g) { return stat(g).rstd; });
+    a.bias = b;
+#pragma unroll
+    for (int i = 0; i < 4; i++) a.scale.p[i] = mul2(w.p[i], rstd[i]);
+    return a;
+}
+
+// y (and the checkpoint) of the feed's rows of this thread's unit, last batch
+// first; row0 is the first of the `phase_has` rows of its phase (a thread without
+// a unit has rows too: its lane may write a block's scale).
 template <class T, int AW, bool kSame, bool kKeep>
-__device__ __forceinline__ void apply_rows(const Batch& B, int n, int r0, int r1, int phase,
-                                           int unit, int cnt, bool on, const PerGroup<kSame>& mean,
-                                           const V8& scale, const V8& bias,
-                                           const Raw<T>* kept_rows) {
-    constexpr int U = kOutRows<T>;
-    const int most = (r1 - r0 + B.phases - 1) / B.phases;
-    if (most <= 0) return;
-    const int rows = phase < B.phases ? (r1 - r0 - phase + B.phases - 1) / B.phases : 0;
-    int it = (most - 1) / U * U;
-    const int64_t row = r0 + phase + (int64_t)it * B.phases;
-    const T* x = (const T*)B.x + n * B.xs + row * B.xr + unit * kUnit;
-    T* y = (T*)B.out + n * B.os + row * B.orow + unit * kUnit;
-    const int64_t xstep = B.phases * B.xr, ystep = B.phases * B.orow;
+__device__ __forceinline__ void apply_rows(const Batch& B, const Feed<FwdRow<T>>& feed,
+                                           const FwdRow<T>& rows, int n, int row0, int phase_has,
+                                           int unit, int cnt, bool on, const Affine<kSame>& q) {
+    constexpr int U = FwdRow<T>::kRows, S = FwdRow<T>::kBytes * kThreads;
+    const int64_t last = row0 + (int64_t)(feed.batches - 1) * U * B.phases;
+    T* y = (T*)B.out + n * B.os + last * B.orow + unit * kUnit;
+    const int64_t ystep = B.phases * B.orow;
     KeptAt kept;
-    if (kKeep) kept = kept_at(B.kept, (int64_t)n * B.s + row, B.phases, unit);
-    for (; it >= 0; it -= U) {
-        bool live[U];
+    if (kKeep) kept = kept_at(B.kept, (int64_t)n * B.s + last, B.phases, unit);
+    feed.template backward<AW>(rows, cnt, [&](uint32_t slot, int first) {
         Raw<T> raw[U] = {};
+        bool live[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) live[u] = it + u < rows;
-        if (it + U <= B.keep) {
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                if (on && live[u]) raw[u] = kept_rows[(it + u) * kThreads + threadIdx.x];
-        } else {
-            const T* at = x;
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (on && live[u]) raw[u] = ld_unit<T, AW>(at, cnt);
-                at += xstep;
-            }
+        for (int j = 0; j < U; j++) {
+            live[j] = first + j < phase_has;
+            if (kKeep && on && live[j]) raw[j] = shared_unit<T>(slot + j * S);
         }
         T* to = y;
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (on && live[u]) {
-                V8 v = unpack(raw[u]);
+        for (int j = 0; j < U; j++) {
+            if (on && live[j]) {
+                V8 v = unpack(kKeep ? raw[j] : shared_unit<T>(slot + j * S));
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    v.p[i] = fma2(sub2(v.p[i], mean[i]), scale.p[i], bias.p[i]);
+                    v.p[i] = fma2(add2(v.p[i], q.minus[i]), q.scale.p[i], q.bias.p[i]);
                 activate<sizeof(T) == 2>(v, B.act, B.param);
                 Raw<T> o;
                 pack(v, o);
@@ -343,24 +629,17 @@ __device__ __forceinline__ void apply_rows(const Batch& B, int n, int r0, int r1
             kept.codes -= U * kept.codes_step;
             kept.scale -= U * kept.scale_step;
         }
-        x -= U * xstep;
         y -= U * ystep;
-    }
+    });
 }
 
 // ---- forward in one launch: a cluster per slab of a sample -------------------------------
 
 template <class T, int AW, bool kSame, bool kKeep>
-__global__ void __launch_bounds__(kThreads, 2) k_norm(Batch B) {
+__global__ void __launch_bounds__(kThreads, kBlocks) k_norm(Batch B) {
     constexpr int E = kSame ? 1 : 8;
     extern __shared__ uint4 dyn[];
-    __shared__ float cnt_sm[2 * kThreads];
-    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile, width = B.tile * E;
-    Raw<T>* rows_sm = reinterpret_cast<Raw<T>*>(dyn);
-    float2* stat = reinterpret_cast<float2*>(rows_sm + B.keep * kThreads);  // mean, rstd
-    Moments* red = reinterpret_cast<Moments*>(stat + B.slab / B.d);
-    Moments* own = red + B.phases * width;                                  // this block's groups
-
+    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
     const int rank = (int)cluster_rank();
     const int id = blockIdx.x / B.chunks, n = id / B.slabs, c0 = id % B.slabs * B.slab;
     const int cw = min(B.slab, B.c - c0), groups = cw / B.d, g0 = c0 / B.d;
@@ -370,99 +649,110 @@ __global__ void __launch_bounds__(kThreads, 2) k_norm(Batch B) {
     const int unit = c0 / kUnit + u, cnt = min(kUnit, c0 + cw - unit * kUnit);
     const bool on = phase < B.phases && u * kUnit < cw;
 
-    Moments m[E] = {};
-    int rows = 0;
-    if (on)
-        rows = unit_moments<T, AW, kSame>(
-            (const T*)B.x + (int64_t)n * B.xs + unit * kUnit, B.xr, r0 + phase, r1, B.phases, cnt,
-            m, [&](int it, const Raw<T>& raw) {
-                if (it < B.keep) rows_sm[it * kThreads + threadIdx.x] = raw;
-            });
-    V8 scale = ld_params(on ? B.w : nullptr, B.ptype, unit * kUnit, cnt, 1.0f);
-    const V8 bias = ld_params(on ? B.b : nullptr, B.ptype, unit * kUnit, cnt, 0.0f);
-    if (phase < B.phases) {
-#pragma unroll
-        for (int i = 0; i < E; i++) red[phase * width + u * E + i] = m[i];
-        if (u == 0) cnt_sm[phase] = (float)(rows * (kSame ? kUnit : 1));
-    }
+    using Row = FwdRow<T>;
+    const int most = (r1 - r0 + B.phases - 1) / B.phases;
+    const Feed<Row> feed(B, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0);
+    const int places = B.keep + (B.keep_all ? 0 : B.ahead);
+    float* sums_at = reinterpret_cast<float*>((char*)dyn + (int64_t)places * Row::kRows *
+                                                              Row::kBytes * kThreads);
+    const CellSums sums(sums_at, B.phases, B.tile * E, kSame);
+    Moments* own = reinterpret_cast<Moments*>(sums_at + cell_floats(B.phases, B.tile * E, kSame));
+    Stat* stat = reinterpret_cast<Stat*>(own + B.slab / B.d);
+    const Row rows(B, n, r0 + phase, unit);
+
+    if (phase < B.phases) sum_rows<T, AW, kSame>(feed, rows, cnt, sums, phase, u);
+    const V8 w = ld_params(on ? B.w : nullptr, B.ptype, unit * kUnit, cnt, 1.0f);
+    const V8 b = ld_params(on ? B.b : nullptr, B.ptype, unit * kUnit, cnt, 0.0f);
     __syncthreads();
-    join_phases<E>(red, cnt_sm, B.phases, width, phase, u * E);
-    const int cells = kSame ? B.d / kUnit : B.d, per = kSame ? kUnit : 1;
-    group_moments(red, groups, cells, (float)(r1 - r0) * per,
-                  [&](int g, Moments q) { own[g] = q; });
+    join_groups(sums, B.phases, r1 - r0, 0, kSame ? cw / kUnit : cw, kSame ? B.d / kUnit : B.d,
+                kSame ? kUnit : 1, [&](int g, float, Moments m) { own[g] = m; });
     cluster_arrive();
     cluster_wait();
-    for (int g = threadIdx.x; g < groups; g += kThreads) {
+    // A group's blocks on neighbouring lanes, joined pairwise.
+    for (int base = 0; base < groups; base += kThreads / kCluster) {
+        const int g = base + threadIdx.x / kCluster, k = threadIdx.x % kCluster;
         Moments q = {0.0f, 0.0f, 0.0f};
         float have = 0.0f;
-        for (int k = 0; k < B.chunks; k++) {
-            int a, b;
-            chunk_rows(len, B.chunks, k, a, b);
-            const float c = (float)(b - a) * (float)B.d;
-            const Moments o = {ld_cluster(&own[g].k, k), ld_cluster(&own[g].off, k),
-                               ld_cluster(&own[g].m2, k)};
-            if (c > 0.0f) q = join(have, q, c, o);
-            have += c;
+        if (g < groups && k < B.chunks) {
+            int a, e;
+            chunk_rows(len, B.chunks, k, a, e);
+            have = (float)(e - a) * (float)B.d;
+            q = {ld_cluster(&own[g].k, k), ld_cluster(&own[g].off, k), ld_cluster(&own[g].m2, k)};
         }
-        const float mu = q.k + q.off, var = have > 0.0f ? q.m2 / have : 0.0f;
-        const float rs = __fdiv_rn(1.0f, __fsqrt_rn(var + B.eps));
-        stat[g] = make_float2(mu, rs);
-        if (rank == 0) {
-            const int64_t at = (int64_t)n * B.g + g0 + g;
-            if (B.mean_out) B.mean_out[at] = mu;
-            if (B.rstd_out) B.rstd_out[at] = rs;
+#pragma unroll
+        for (int o = kCluster / 2; o; o /= 2) {
+            const float more = __shfl_down_sync(~0u, have, o, kCluster);
+            const Moments m = {__shfl_down_sync(~0u, q.k, o, kCluster),
+                               __shfl_down_sync(~0u, q.off, o, kCluster),
+                               __shfl_down_sync(~0u, q.m2, o, kCluster)};
+            q = join(have, q, more, m);
+            have += more;
+        }
+        if (g < groups && k == 0) {
+            const float mu = len ? q.k + q.off : 0.0f, var = have > 0.0f ? q.m2 / have : 0.0f;
+            const float rs = __fdiv_rn(1.0f, __fsqrt_rn(var + B.eps));
+            stat[g] = {mu, rs};
+            if (rank == 0) {
+                const int64_t at = (int64_t)n * B.g + g0 + g;
+                if (B.mean_out) B.mean_out[at] = mu;
+                if (B.rstd_out) B.rstd_out[at] = rs;
+            }
         }
     }
     cluster_arrive();  // the others' shared memory has been read
     __syncthreads();
-    const int last = c0 + cw - 1, first = min(unit * kUnit, last);
-    const auto mean = per_group<kSame>(first, last, B.d, [&](int g) { return stat[g - g0].x; });
-    const auto rstd = per_group<kSame>(first, last, B.d, [&](int g) { return stat[g - g0].y; });
-#pragma unroll
-    for (int i = 0; i < 4; i++) scale.p[i] = mul2(scale.p[i], rstd[i]);
-    apply_rows<T, AW, kSame, kKeep>(B, n, r0, r1, phase, unit, cnt, on, mean, scale, bias, rows_sm);
+    const int last = c0 + cw - 1;
+    const auto q = affine<kSame>(B, w, b, min(unit * kUnit, last), last,
+                                 [&](int g) { return stat[g - g0]; });
+    apply_rows<T, AW, kSame, kKeep>(B, feed, rows, n, r0 + phase, phase_rows(B, r0, r1, phase),
+                                    unit, cnt, on, q);
     cluster_wait();
 }
 
 // ---- forward over chunks: moments, joined, then applied ---------------------------
 
 template <class T, int AW, bool kSame>
-__global__ void __launch_bounds__(kThreads, 2) k_stats(Batch B, Moments* __restrict__ part) {
+__global__ void __launch_bounds__(kThreads, kBlocks) k_stats(Batch B, Moments* part) {
     constexpr int E = kSame ? 1 : 8;
-    extern __shared__ Moments sm[];
-    __shared__ float cnt_sm[2 * kThreads];
-    Moments* cell_m = sm;                         // every cell of the row
-    Moments* red = sm + (int64_t)B.units * E;     // phases * tile * E
+    extern __shared__ uint4 dyn[];
+    // A group that a tile's end cuts is carried to the next tile.
+    __shared__ Moments carry[2];
+    __shared__ float carried[2];
+    using Row = FwdRow<T>;
+    float* sums_at = reinterpret_cast<float*>((char*)dyn + (int64_t)B.ahead * Row::kRows *
+                                                              Row::kBytes * kThreads);
+    const CellSums sums(sums_at, B.phases, B.tile * E, kSame);
     const int n = blockIdx.x / B.chunks, k = blockIdx.x % B.chunks;
     int r0, r1;
     chunk_rows(valid_rows(B, n), B.chunks, k, r0, r1);
-    const T* x = (const T*)B.x + (int64_t)n * B.xs;
-    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile, width = B.tile * E;
+    Moments* o = part + ((int64_t)n * B.chunks + k) * B.g;
+    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
+    const int most = (r1 - r0 + B.phases - 1) / B.phases;
+    const int cells = kSame ? B.c / kUnit : B.c, d = kSame ? B.d / kUnit : B.d;
     for (int t = 0; t < B.tiles; t++) {
-        const int unit = t * B.tile + u;
-        if (phase < B.phases) {
-            Moments m[E] = {};
-            int rows = 0;
-            if (unit < B.units)
-                rows = unit_moments<T, AW, kSame>(x + unit * kUnit, B.xr, r0 + phase, r1, B.phases,
-                                                  min(kUnit, B.c - unit * kUnit), m,
-                                                  [](int, const Raw<T>&) {});
-#pragma unroll
-            for (int i = 0; i < E; i++) red[phase * width + u * E + i] = m[i];
-            if (u == 0) cnt_sm[phase] = (float)(rows * (kSame ? kUnit : 1));
-        }
+        const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
+        const bool on = phase < B.phases && unit < B.units;
+        const Feed<Row> feed(B, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0);
+        if (phase < B.phases)
+            sum_rows<T, AW, kSame>(feed, Row(B, n, r0 + phase, unit), cnt, sums, phase, u);
         __syncthreads();
-        join_phases<E>(red, cnt_sm, B.phases, width, phase, u * E);
-        if (phase == 0 && unit < B.units) {
-#pragma unroll
-            for (int i = 0; i < E; i++) cell_m[unit * E + i] = red[u * E + i];
-        }
+        if (t == B.tiles - 1) grid_release();
+        const int t0 = t * B.tile * E, t1 = min(t0 + B.tile * E, cells), odd = t & 1;
+        join_groups(sums, B.phases, r1 - r0, t0, t1, d, kSame ? kUnit : 1,
+                    [&](int g, float count, Moments m) {
+                        if (g * d < t0) {
+                            m = join(carried[odd ^ 1], carry[odd ^ 1], count, m);
+                            count += carried[odd ^ 1];
+                        }
+                        if (g * d + d > t1) {
+                            carry[odd] = m;
+                            carried[odd] = count;
+                        } else {
+                            o[g] = m;
+                        }
+                    });
         __syncthreads();
     }
-    grid_release();
-    Moments* o = part + ((int64_t)n * B.chunks + k) * B.g;
-    group_moments(cell_m, B.g, kSame ? B.d / kUnit : B.d, (float)(r1 - r0) * (kSame ? kUnit : 1),
-                  [&](int g, Moments m) { o[g] = m; });
 }
 
 // A block joins the chunks of up to `wide` groups of a sample: its threads take
@@ -470,25 +760,30 @@ __global__ void __launch_bounds__(kThreads, 2) k_stats(Batch B, Moments* __restr
 // chunk's mean, so one pass over the parts serves both moments.
 constexpr int kJoin = 512;
 __global__ void __launch_bounds__(kJoin)
-    k_join(Batch B, const Moments* __restrict__ part, int wide, int blocks) {
+    k_join(Batch B, const Moments* part, int wide, int blocks) {
     __shared__ double s1[kJoin], s2[kJoin];
     grid_wait();
     const int n = blockIdx.x / blocks, g = blockIdx.x % blocks * wide + threadIdx.x % wide;
     const int lane = threadIdx.x / wide, lanes = kJoin / wide;
-    const int len = valid_rows(B, n);
+    const int len = valid_rows(B, n), per = (len + B.chunks - 1) / B.chunks;
     double a = 0.0, q = 0.0, ref = 0.0;
     if (g < B.g) {
         const Moments* p = part + (int64_t)n * B.chunks * B.g + g;
         ref = (double)p[0].k + p[0].off;
-#pragma unroll 4
-        for (int k = lane; k < B.chunks; k += lanes) {
-            int r0, r1;
-            chunk_rows(len, B.chunks, k, r0, r1);
-            const Moments m = p[(int64_t)k * B.g];
-            const double c = (double)(r1 - r0) * B.d, dv = ((double)m.k + m.off) - ref;
-            if (r1 > r0) {
-                a += c * dv;
-                q += m.m2 + c * dv * dv;
+        for (int k = lane; k < B.chunks; k += 4 * lanes) {
+            Moments m[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (k + j * lanes < B.chunks) m[j] = p[(int64_t)(k + j * lanes) * B.g];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int64_t first = (int64_t)(k + j * lanes) * per;
+                const int64_t have = min((int64_t)per, len - first);
+                if (k + j * lanes < B.chunks && have > 0) {
+                    const double c = (double)have * B.d, dv = ((double)m[j].k - ref) + m[j].off;
+                    a += c * dv;
+                    q += m[j].m2 + c * dv * dv;
+                }
             }
         }
     }
@@ -514,117 +809,36 @@ __global__ void __launch_bounds__(kJoin)
 }
 
 template <class T, int AW, bool kSame, bool kKeep>
-__global__ void __launch_bounds__(kThreads, 2) k_apply(Batch B) {
+__global__ void __launch_bounds__(kThreads, kBlocks) k_apply(Batch B) {
+    extern __shared__ uint4 dyn[];
     grid_wait();
     const int id = gridDim.x - 1 - blockIdx.x, n = id / B.chunks;
     int r0, r1;
     chunk_rows(valid_rows(B, n), B.chunks, id % B.chunks, r0, r1);
     if (r0 >= r1) return;
+    using Row = FwdRow<T>;
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
+    const int most = (r1 - r0 + B.phases - 1) / B.phases;
     const float *mu = B.mean_out + (int64_t)n * B.g, *rs = B.rstd_out + (int64_t)n * B.g;
     for (int t = 0; t < B.tiles; t++) {
         const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
         const bool on = phase < B.phases && unit < B.units;
-        const int first = min(unit * kUnit, B.c - 1);
-        const auto mean = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return mu[g]; });
-        const auto rstd = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return rs[g]; });
-        V8 scale = ld_params(on ? B.w : nullptr, B.ptype, unit * kUnit, cnt, 1.0f);
-        const V8 bias = ld_params(on ? B.b : nullptr, B.ptype, unit * kUnit, cnt, 0.0f);
-#pragma unroll
-        for (int i = 0; i < 4; i++) scale.p[i] = mul2(scale.p[i], rstd[i]);
-        apply_rows<T, AW, kSame, kKeep>(B, n, r0, r1, phase, unit, cnt, on, mean, scale, bias,
-                                        nullptr);
+        const Feed<Row> feed(B, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0);
+        const V8 w = ld_params(on ? B.w : nullptr, B.ptype, unit * kUnit, cnt, 1.0f);
+        const V8 b = ld_params(on ? B.b : nullptr, B.ptype, unit * kUnit, cnt, 0.0f);
+        const auto q = affine<kSame>(B, w, b, min(unit * kUnit, B.c - 1), B.c - 1, [&](int g) {
+            return Stat{mu[g], rs[g]};
+        });
+        apply_rows<T, AW, kSame, kKeep>(B, feed, Row(B, n, r0 + phase, unit), n, r0 + phase,
+                                        phase_rows(B, r0, r1, phase), unit, cnt, on, q);
     }
 }
 
 // ---- backward ---------------------------------------------------------------------
 
-// A unit of x and of dy, x from the tensor or from its checkpoint.
-template <class T, int AW, bool kFrom>
-struct Pair {
-    Raw<T> dy, x;
-    Codes codes;
-    float scale;
-    __device__ __forceinline__ V8 input() const { return kFrom ? decode(codes, scale) : unpack(x); }
-};
-// A thread's walk along its rows of both.
-template <class T, int AW, bool kFrom>
-struct PairWalk {
-    const T *dy, *x;
-    KeptAt kept;
-    int64_t dy_step, x_step;
-    __device__ __forceinline__ PairWalk(const Batch& B, int n, int64_t row, int unit) {
-        dy = (const T*)B.dy + n * B.ys + row * B.yr + unit * kUnit;
-        dy_step = B.phases * B.yr;
-        if (kFrom) {
-            kept = kept_at(B.kept, (int64_t)n * B.s + row, B.phases, unit);
-        } else {
-            x = (const T*)B.x + n * B.xs + row * B.xr + unit * kUnit;
-            x_step = B.phases * B.xr;
-        }
-    }
-    __device__ __forceinline__ void load(Pair<T, AW, kFrom>& v, int cnt) const {
-        v.dy = ld_unit<T, AW>(dy, cnt);
-        if (kFrom) {
-            v.codes = ld_codes<AW == 16>(kept.codes, cnt);
-            v.scale = __ldg(kept.scale);
-        } else {
-            v.x = ld_unit<T, AW>(x, cnt);
-        }
-    }
-    __device__ __forceinline__ void move(int rows) {
-        dy += rows * dy_step;
-        if (kFrom) {
-            kept.codes += rows * kept.codes_step;
-            kept.scale += rows * kept.scale_step;
-        } else {
-            x += rows * x_step;
-        }
-    }
-};
-// The same in shared memory: arrays of iterations by threads.
-template <class T, bool kFrom>
-struct PairStore {
-    Raw<T>* dy;
-    Raw<T>* x;
-    uint2* codes;
-    float* scale;
-    static constexpr int kBytes = (int)sizeof(Raw<T>) + (kFrom ? 12 : (int)sizeof(Raw<T>));
-    __device__ __forceinline__ PairStore(void* base, int iters) {
-        char* p = (char*)base;
-        const int64_t cells = (int64_t)iters * kThreads;
-        dy = (Raw<T>*)p;
-        x = (Raw<T>*)(p + cells * sizeof(Raw<T>));
-        codes = (uint2*)x;
-        scale = (float*)(codes + cells);
-    }
-    template <int AW>
-    __device__ __forceinline__ void put(int it, const Pair<T, AW, kFrom>& v) {
-        const int at = it * kThreads + threadIdx.x;
-        dy[at] = v.dy;
-        if (kFrom) {
-            codes[at] = v.codes.q;
-            scale[at] = v.scale;
-        } else {
-            x[at] = v.x;
-        }
-    }
-    template <int AW>
-    __device__ __forceinline__ void get(int it, Pair<T, AW, kFrom>& v) const {
-        const int at = it * kThreads + threadIdx.x;
-        v.dy = dy[at];
-        if (kFrom) {
-            v.codes.q = codes[at];
-            v.scale = scale[at];
-        } else {
-            v.x = x[at];
-        }
-    }
-};
-
 template <bool kSame>
 struct BackParams {
-    PerGroup<kSame> mean, rstd;
+    PerGroup<kSame> minus, rstd;  // the mean negated
     V8 w, b;
 };
 template <bool kSame>
@@ -633,93 +847,108 @@ __device__ __forceinline__ BackParams<kSame> back_params(const Batch& B, int n, 
     BackParams<kSame> q;
     const int first = min(unit * kUnit, B.c - 1);
     const float *mu = B.mean + (int64_t)n * B.g, *rs = B.rstd + (int64_t)n * B.g;
-    q.mean = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return __ldg(mu + g); });
+    q.minus = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return -__ldg(mu + g); });
     q.rstd = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return __ldg(rs + g); });
     q.w = ld_params(on ? B.w : nullptr, B.ptype, unit * kUnit, cnt, 1.0f);
     q.b = ld_params(on ? B.b : nullptr, B.ptype, unit * kUnit, cnt, 0.0f);
     return q;
 }
 
-// xh and dz = dy * act'(z) of one unit.
-template <class T, int AW, bool kFrom, bool kSame>
-__device__ __forceinline__ void slopes(const Batch& B, const BackParams<kSame>& q,
-                                       const Pair<T, AW, kFrom>& in, V8& xh, V8& dz) {
-    V8 z, f;
-    xh = in.input();
+// xh and dz = dy * act'(z) of the unit in a slot.
+template <class T, bool kFrom, bool kSame>
+__device__ __forceinline__ void slopes(const Batch& B, const BackParams<kSame>& q, uint32_t slot,
+                                       V8& xh, V8& dz) {
+    xh = BackRow<T, kFrom>::input(slot);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        xh.p[i] = mul2(sub2(xh.p[i], q.mean[i]), q.rstd[i]);
-        z.p[i] = fma2(xh.p[i], q.w.p[i], q.b.p[i]);
-    }
-    const V8 g = unpack(in.dy);
+    for (int i = 0; i < 4; i++) xh.p[i] = mul2(add2(xh.p[i], q.minus[i]), q.rstd[i]);
+    const V8 g = unpack(shared_unit<T>(slot));
     if (B.act == SIMTGO_ACT_NONE) {
         dz = g;
         return;
     }
+    V8 z, f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) z.p[i] = fma2(xh.p[i], q.w.p[i], q.b.p[i]);
     activate_slope<sizeof(T) == 2>(z, f, dz, B.act, B.param);
 #pragma unroll
     for (int i = 0; i < 4; i++) dz.p[i] = mul2(dz.p[i], g.p[i]);
 }
 
-// Sums A = dz and C = dz*xh of the unit's channels over the thread's rows.
-template <class T, int AW, bool kFrom, bool kSame, class F>
-__device__ __forceinline__ void back_sums(const Batch& B, const BackParams<kSame>& q, int n, int r,
-                                          int r1, int unit, int cnt, float2 (&a)[4], float2 (&c)[4],
-                                          F&& keep) {
-    constexpr int U = kOutRows<T>;
-    const int rows = (r1 - r + B.phases - 1) / B.phases;
-    PairWalk<T, AW, kFrom> walk(B, n, r, unit);
-    for (int it = 0; it < rows; it += U) {
-        Pair<T, AW, kFrom> in[U];
-#pragma unroll
-        for (int j = 0; j < U; j++) {
-            if (it + j < rows) walk.load(in[j], cnt);
-            walk.move(1);
-        }
-#pragma unroll
-        for (int j = 0; j < U; j++)
-            if (it + j < rows) {
-                keep(it + j, in[j]);
-                V8 xh, dz;
-                slopes(B, q, in[j], xh, dz);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    a[i] = add2(a[i], dz.p[i]);
-                    c[i] = fma2(dz.p[i], xh.p[i], c[i]);
-                }
-            }
+// A = sum dz and B = sum dz*xh of every channel over the phases, in shared memory.
+struct ChannelSums {
+    float *a, *b;      // of a phase
+    float2 *half, *all;  // of some of the phases; of all
+    int width;
+    __device__ __forceinline__ ChannelSums(void* base, int phases, int channels)
+        : width(channels + 4) {
+        a = (float*)base;
+        b = a + phases * width;
+        half = reinterpret_cast<float2*>(b + phases * width);
+        all = half + kThreads;
     }
+};
+__host__ __device__ constexpr int channel_bytes(int phases, int channels) {
+    return 8 * phases * (channels + 4) + 8 * kThreads + 8 * channels;
 }
 
-// Adds the phases' (A, B) of every channel; phase 0 ends with the sums. Every
-// thread calls it; it begins with a barrier.
-__device__ __forceinline__ void add_phases(float2* red, int phases, int width, int phase, int u,
-                                           const float2 (&a)[4], const float2 (&b)[4]) {
-    // (A, A, B, B) of two channels at a time: 16 bytes a thread.
-    float4* mine = reinterpret_cast<float4*>(red + phase * width) + u * 4;
-    if (phase < phases) {
+// Sums the thread's rows and then the block's phases into sums.all. Every
+// thread calls it; ends with a barrier.
+template <class T, int AW, bool kFrom, bool kSame>
+__device__ __forceinline__ void back_sums(const Batch& B, const Feed<BackRow<T, kFrom>>& feed,
+                                          const BackRow<T, kFrom>& rows,
+                                          const BackParams<kSame>& q, const ChannelSums& sums,
+                                          int phase, int u, int cnt) {
+    using Row = BackRow<T, kFrom>;
+    const int channels = B.tile * kUnit;
+    if (phase < B.phases) {
+        float2 a[4] = {}, b[4] = {};
+        feed.template forward<AW>(rows, cnt, [&](uint32_t slot, int first) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) mine[i] = make_float4(a[i].x, a[i].y, b[i].x, b[i].y);
+            for (int j = 0; j < Row::kRows; j++)
+                if (first + j < feed.mine) {
+                    V8 xh, dz;
+                    slopes<T, kFrom>(B, q, slot + j * Row::kBytes * kThreads, xh, dz);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        a[i] = add2(a[i], dz.p[i]);
+                        b[i] = fma2(dz.p[i], xh.p[i], b[i]);
+                    }
+                }
+        });
+        const int at = phase * sums.width + u * kUnit;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            *reinterpret_cast<float4*>(sums.a + at + 4 * i) =
+                make_float4(a[2 * i].x, a[2 * i].y, a[2 * i + 1].x, a[2 * i + 1].y);
+            *reinterpret_cast<float4*>(sums.b + at + 4 * i) =
+                make_float4(b[2 * i].x, b[2 * i].y, b[2 * i + 1].x, b[2 * i + 1].y);
+        }
     }
     __syncthreads();
-    for (int m = phases; m > 1;) {
-        const int h = (m + 1) / 2;
-        if (phase + h < m) {
-            const float4* o = reinterpret_cast<const float4*>(red + (phase + h) * width) + u * 4;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float4 v = o[i], w = mine[i];
-                mine[i] = make_float4(w.x + v.x, w.y + v.y, w.z + v.z, w.w + v.w);
-            }
+    // Several threads to a channel where there are fewer channels than threads.
+    const int split = max(1, min(kThreads / channels, B.phases));
+    for (int i = threadIdx.x; i < split * channels; i += kThreads) {
+        const int c = i % channels;
+        float x = 0.0f, y = 0.0f;
+#pragma unroll 4
+        for (int p = i / channels; p < B.phases; p += split) {
+            x += sums.a[p * sums.width + c];
+            y += sums.b[p * sums.width + c];
         }
-        m = h;
+        (split > 1 ? sums.half : sums.all)[i] = make_float2(x, y);
+    }
+    __syncthreads();
+    if (split > 1) {
+        for (int c = threadIdx.x; c < channels; c += kThreads) {
+            float2 v = sums.half[c];
+            for (int k = 1; k < split; k++) {
+                v.x += sums.half[k * channels + c].x;
+                v.y += sums.half[k * channels + c].y;
+            }
+            sums.all[c] = v;
+        }
         __syncthreads();
     }
-}
-// Channel i's (A, B) after add_phases.
-__device__ __forceinline__ float2 channel_sum(const float2* red, int i) {
-    const float4 v = reinterpret_cast<const float4*>(red)[i / 2];
-    return i & 1 ? make_float2(v.y, v.w) : make_float2(v.x, v.z);
 }
 
 // sum of w*A and w*B over each group's d channels, at(i) giving channel i's
@@ -747,68 +976,50 @@ __device__ __forceinline__ void group_sums(const Batch& B, int c0, int groups, A
     }
 }
 
-// dx of rows [r0, r1) of this thread's unit, last rows first. s1 and s2 are the
-// negated means, added.
+// dx of the feed's rows of this thread's unit, last batch first, from the
+// negated means s1 of dz*w and s2 of dz*w*xh.
 template <class T, int AW, bool kFrom, bool kSame>
-__device__ __forceinline__ void back_rows(const Batch& B, const BackParams<kSame>& q,
-                                          const PerGroup<kSame>& s1, const PerGroup<kSame>& s2,
-                                          int n, int r0, int r1, int phase, int unit, int cnt,
-                                          const PairStore<T, kFrom>& store) {
-    constexpr int U = kOutRows<T>;
-    const int rows = (r1 - r0 - phase + B.phases - 1) / B.phases;
-    if (rows <= 0) return;
-    int it = (rows - 1) / U * U;
-    const int64_t row = r0 + phase + (int64_t)it * B.phases;
-    PairWalk<T, AW, kFrom> walk(B, n, row, unit);
-    T* dx = (T*)B.out + n * B.os + row * B.orow + unit * kUnit;
+__device__ __forceinline__ void back_rows(const Batch& B, const Feed<BackRow<T, kFrom>>& feed,
+                                          const BackRow<T, kFrom>& rows,
+                                          const BackParams<kSame>& q, const PerGroup<kSame>& s1,
+                                          const PerGroup<kSame>& s2, int n, int row0, int unit,
+                                          int cnt) {
+    using Row = BackRow<T, kFrom>;
+    const int64_t last = row0 + (int64_t)(feed.batches - 1) * Row::kRows * B.phases;
+    T* dx = (T*)B.out + n * B.os + last * B.orow + unit * kUnit;
     const int64_t step = B.phases * B.orow;
-    for (; it >= 0; it -= U) {
-        Pair<T, AW, kFrom> in[U];
-        if (it + U <= B.keep) {
-#pragma unroll
-            for (int j = 0; j < U; j++)
-                if (it + j < rows) store.get(it + j, in[j]);
-            walk.move(-U);
-        } else {
-#pragma unroll
-            for (int j = 0; j < U; j++) {
-                if (it + j < rows) walk.load(in[j], cnt);
-                walk.move(1);
-            }
-            walk.move(-2 * U);
-        }
+    feed.template backward<AW>(rows, cnt, [&](uint32_t slot, int first) {
         T* to = dx;
 #pragma unroll
-        for (int j = 0; j < U; j++) {
-            if (it + j < rows) {
+        for (int j = 0; j < Row::kRows; j++) {
+            if (first + j < feed.mine) {
                 V8 xh, dz;
-                slopes(B, q, in[j], xh, dz);
+                slopes<T, kFrom>(B, q, slot + j * Row::kBytes * kThreads, xh, dz);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 v = fma2(dz.p[i], q.w.p[i], s1[i]);
-                    dz.p[i] = mul2(q.rstd[i], fma2(xh.p[i], s2[i], v));
-                }
+                for (int i = 0; i < 4; i++)
+                    dz.p[i] = mul2(q.rstd[i], fma2(xh.p[i], s2[i], fma2(dz.p[i], q.w.p[i], s1[i])));
                 Raw<T> o;
                 pack(dz, o);
                 st_unit<T, AW>(to, o, cnt);
             }
             to += step;
         }
-        dx -= U * step;
-    }
+        dx -= Row::kRows * step;
+    });
 }
 
 // One launch for dx: a cluster per slab of a sample. part, where wanted,
 // receives every block's (A, B) of its channels, for k_back_join.
 template <class T, int AW, bool kFrom, bool kSame>
-__global__ void __launch_bounds__(kThreads, 2) k_norm_back(Batch B, float2* __restrict__ part) {
+__global__ void __launch_bounds__(kThreads, kBackBlocks) k_norm_back(Batch B, float2* part) {
     extern __shared__ uint4 dyn[];
-    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile, width = B.tile * kUnit;
-    PairStore<T, kFrom> store(dyn, B.keep);
-    float2* red = reinterpret_cast<float2*>(
-        (char*)dyn + (int64_t)B.keep * kThreads * PairStore<T, kFrom>::kBytes);
-    float2* own = red + B.phases * width;     // this block's group sums
-    float2* means = own + B.slab / B.d;       // the cluster's, over the count
+    using Row = BackRow<T, kFrom>;
+    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
+    const int places = B.keep + (B.keep_all ? 0 : B.ahead);
+    const ChannelSums sums((char*)dyn + (int64_t)places * Row::kRows * Row::kBytes * kThreads,
+                           B.phases, B.tile * kUnit);
+    float2* own = sums.all + B.tile * kUnit;  // this block's group sums
+    float2* means = own + B.slab / B.d;       // the cluster's, over the count, negated
 
     const int rank = (int)cluster_rank();
     const int id = blockIdx.x / B.chunks, n = id / B.slabs, c0 = id % B.slabs * B.slab;
@@ -820,66 +1031,68 @@ __global__ void __launch_bounds__(kThreads, 2) k_norm_back(Batch B, float2* __re
     const bool on = phase < B.phases && u * kUnit < cw;
 
     const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, on);
-    float2 a[4] = {}, b[4] = {};
-    if (on)
-        back_sums<T, AW, kFrom>(B, q, n, r0 + phase, r1, unit, cnt, a, b,
-                                [&](int it, const Pair<T, AW, kFrom>& v) {
-                                    if (it < B.keep) store.put(it, v);
-                                });
-    add_phases(red, B.phases, width, phase, u, a, b);
+    const int most = (r1 - r0 + B.phases - 1) / B.phases;
+    const Feed<Row> feed(B, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0);
+    const Row rows(B, n, r0 + phase, unit);
+    back_sums<T, AW, kFrom, kSame>(B, feed, rows, q, sums, phase, u, cnt);
     if (part)
         for (int i = threadIdx.x; i < cw; i += kThreads)
-            part[((int64_t)n * B.chunks + rank) * B.c + c0 + i] = channel_sum(red, i);
+            part[((int64_t)n * B.chunks + rank) * B.c + c0 + i] = sums.all[i];
     grid_release();
     if (!B.out) return;  // the same for every block of the grid
-    group_sums(B, c0, groups, [&](int i) { return channel_sum(red, i); },
+    group_sums(B, c0, groups, [&](int i) { return sums.all[i]; },
                [&](int g, float2 v) { own[g] = v; });
     cluster_arrive();
     cluster_wait();
-    for (int g = threadIdx.x; g < groups; g += kThreads) {
+    for (int base = 0; base < groups; base += kThreads / kCluster) {
+        const int g = base + threadIdx.x / kCluster, k = threadIdx.x % kCluster;
         float x = 0.0f, y = 0.0f;
-        for (int k = 0; k < B.chunks; k++) {
-            x += ld_cluster(&own[g].x, k);
-            y += ld_cluster(&own[g].y, k);
+        if (g < groups && k < B.chunks) {
+            x = ld_cluster(&own[g].x, k);
+            y = ld_cluster(&own[g].y, k);
+        }
+#pragma unroll
+        for (int o = kCluster / 2; o; o /= 2) {
+            x += __shfl_down_sync(~0u, x, o, kCluster);
+            y += __shfl_down_sync(~0u, y, o, kCluster);
         }
         const float inv = len ? -1.0f / ((float)len * (float)B.d) : 0.0f;
-        means[g] = make_float2(x * inv, y * inv);
+        if (g < groups && k == 0) means[g] = make_float2(x * inv, y * inv);
     }
-    cluster_arrive();
+    cluster_arrive();  // the others' shared memory has been read
     __syncthreads();
     if (on) {
         const int last = c0 + cw - 1, first = min(unit * kUnit, last);
         const auto s1 = per_group<kSame>(first, last, B.d, [&](int g) { return means[g - g0].x; });
         const auto s2 = per_group<kSame>(first, last, B.d, [&](int g) { return means[g - g0].y; });
-        back_rows<T, AW, kFrom, kSame>(B, q, s1, s2, n, r0, r1, phase, unit, cnt, store);
+        back_rows<T, AW, kFrom, kSame>(B, feed, rows, q, s1, s2, n, r0 + phase, unit, cnt);
     }
     cluster_wait();
 }
 
 // Over chunks: (A, B) of every channel of a chunk.
 template <class T, int AW, bool kFrom, bool kSame>
-__global__ void __launch_bounds__(kThreads, 2) k_back_stats(Batch B, float2* __restrict__ part) {
-    extern __shared__ float4 red4[];
-    float2* red = reinterpret_cast<float2*>(red4);
+__global__ void __launch_bounds__(kThreads, kBackBlocks) k_back_stats(Batch B, float2* part) {
+    extern __shared__ uint4 dyn[];
+    using Row = BackRow<T, kFrom>;
+    const ChannelSums sums((char*)dyn + (int64_t)B.ahead * Row::kRows * Row::kBytes * kThreads,
+                           B.phases, B.tile * kUnit);
     const int n = blockIdx.x / B.chunks, k = blockIdx.x % B.chunks;
     int r0, r1;
     chunk_rows(valid_rows(B, n), B.chunks, k, r0, r1);
     float2* o = part + ((int64_t)n * B.chunks + k) * B.c;
-    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile, width = B.tile * kUnit;
+    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
+    const int most = (r1 - r0 + B.phases - 1) / B.phases;
     for (int t = 0; t < B.tiles; t++) {
         const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
         const bool on = phase < B.phases && unit < B.units;
-        float2 a[4] = {}, b[4] = {};
-        if (on && r0 < r1) {
-            const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, on);
-            back_sums<T, AW, kFrom>(B, q, n, r0 + phase, r1, unit, cnt, a, b,
-                                    [](int, const Pair<T, AW, kFrom>&) {});
-        }
-        add_phases(red, B.phases, width, phase, u, a, b);
-        const int c0 = t * width;
-        for (int i = threadIdx.x; i < min(width, B.c - c0); i += kThreads)
-            o[c0 + i] = channel_sum(red, i);
-        __syncthreads();
+        const Feed<Row> feed(B, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0);
+        const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, on);
+        back_sums<T, AW, kFrom, kSame>(B, feed, Row(B, n, r0 + phase, unit), q, sums, phase, u,
+                                       cnt);
+        const int c0 = t * B.tile * kUnit;
+        for (int i = threadIdx.x; i < min(B.tile * kUnit, B.c - c0); i += kThreads)
+            o[c0 + i] = sums.all[i];
     }
     grid_release();
 }
@@ -889,8 +1102,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_back_stats(Batch B, float2* __r
 // 32 channels of a span, its warps the rows in turn.
 constexpr int kAdd = 1024;
 __global__ void __launch_bounds__(kAdd)
-    k_back_join(const float2* __restrict__ part, int64_t rows, int c, int blocks,
-                float2* __restrict__ tot, float* __restrict__ dw, float* __restrict__ db) {
+    k_back_join(const float2* part, int64_t rows, int c, int blocks, float2* tot, float* dw,
+                float* db) {
     __shared__ double2 sm[kAdd / 32][33];
     grid_wait();
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -925,30 +1138,34 @@ __global__ void __launch_bounds__(kAdd)
 }
 
 template <class T, int AW, bool kFrom, bool kSame>
-__global__ void __launch_bounds__(kThreads, 2)
-    k_back_apply(Batch B, const float2* __restrict__ tot) {
-    extern __shared__ float2 means[];  // of every group
+__global__ void __launch_bounds__(kThreads, kBackBlocks) k_back_apply(Batch B, const float2* tot) {
+    extern __shared__ uint4 dyn[];
     grid_wait();
+    using Row = BackRow<T, kFrom>;
+    float2* means = reinterpret_cast<float2*>(  // of every group, negated
+        (char*)dyn + (int64_t)B.ahead * Row::kRows * Row::kBytes * kThreads);
+    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
     const int id = gridDim.x - 1 - blockIdx.x, n = id / B.chunks;
     const int len = valid_rows(B, n);
     int r0, r1;
     chunk_rows(len, B.chunks, id % B.chunks, r0, r1);
     if (r0 >= r1) return;
     const float inv = -1.0f / ((float)len * (float)B.d);
-    group_sums(B, 0, B.g, [&](int i) { return __ldg(tot + (int64_t)n * B.c + i); },
+    group_sums(B, 0, B.g, [&](int i) { return tot[(int64_t)n * B.c + i]; },
                [&](int g, float2 v) { means[g] = make_float2(v.x * inv, v.y * inv); });
     __syncthreads();
-    const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
     if (phase >= B.phases) return;
-    const PairStore<T, kFrom> none(nullptr, 0);
+    const int most = (r1 - r0 + B.phases - 1) / B.phases;
     for (int t = 0; t < B.tiles; t++) {
         const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
         if (unit >= B.units) break;
+        const Feed<Row> feed(B, dyn, most, phase_rows(B, r0, r1, phase));
         const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, true);
         const int first = unit * kUnit;
         const auto s1 = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return means[g].x; });
         const auto s2 = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return means[g].y; });
-        back_rows<T, AW, kFrom, kSame>(B, q, s1, s2, n, r0, r1, phase, unit, cnt, none);
+        back_rows<T, AW, kFrom, kSame>(B, feed, Row(B, n, r0 + phase, unit), q, s1, s2, n,
+                                       r0 + phase, unit, cnt);
     }
 }
 
@@ -1074,16 +1291,24 @@ void tile_units(Batch& B, int units, int lanes) {
     B.phases = kThreads / B.tile;
 }
 
-// How a call goes through its data. `elem` is the bytes of all inputs per
-// element; `sum_rows`, the rows a thread takes at a time; `iter_bytes`, what an
-// iteration of a block's threads keeps; `cell_bytes`, a thread's sums.
+// How a call goes through its data.
 struct Plan {
     bool cluster;
     unsigned grid;
     size_t smem;
 };
+// What a kernel of the call needs: bytes of all inputs per element, rows of a
+// batch and shared bytes of one, and the shared bytes beside the rows for a tile
+// of so many units, phases and groups.
+struct Needs {
+    double elem;
+    int rows;
+    int64_t batch_bytes;
+    size_t (*beside)(int tile, int phases, int groups, bool same);
+    int per_sm;  // blocks an SM's registers hold
+};
 Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool keep_codes,
-               double elem, int sum_rows, int iter_bytes, int cell_bytes, int group_bytes) {
+               const Needs& need) {
     B.n = c.samples;
     B.s = c.positions;
     B.c = c.channels;
@@ -1093,6 +1318,7 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
     B.act = c.act;
     B.param = c.act_param;
     B.eps = c.eps;
+    const bool same = B.d % kUnit == 0;
     const int units = (c.channels + kUnit - 1) / kUnit;
 
     // A slab: whole groups, units and checkpoint blocks; 128 bytes of every row
@@ -1104,7 +1330,8 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
     if (q < c.channels) {
         const int64_t least = 128 / elem_size(c.type);
         slab = (least + q - 1) / q * q;
-        while (2 * slab <= std::min<int64_t>(c.channels, most) && slab * c.positions * elem < 65536)
+        while (2 * slab <= std::min<int64_t>(c.channels, most) &&
+               slab * c.positions * need.elem < 65536)
             slab *= 2;
         slab = std::min<int64_t>(slab, c.channels);
         const int64_t parts = (c.channels + slab - 1) / slab;
@@ -1121,9 +1348,9 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
         t.slab = (int)slab;
         t.slabs = slabs;
         const int64_t clusters = (int64_t)c.samples * slabs;
-        const double bytes = (double)slab * c.positions * elem;
+        const double bytes = (double)slab * c.positions * need.elem;
         int k = 1;
-        while (k < 8 && c.positions / (2 * k) >= t.phases &&
+        while (k < kCluster && c.positions / (2 * k) >= t.phases &&
                (clusters * k < 2 * d.sms || bytes / k > 96 * 1024))
             k *= 2;
         t.chunks = k;
@@ -1132,15 +1359,30 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
         const double us = bytes * clusters / (std::min<double>(clusters * k, 2 * d.sms) * 36e3);
         const double chunked = bytes * clusters / 6.4e6 + 6.0;
         if (us <= chunked && clusters * k <= 0x7fffffff) {
-            const size_t fixed = (size_t)t.phases * t.tile * cell_bytes +
-                                 (size_t)(slab / B.d + 1) * group_bytes + 32;
-            const size_t room = (clusters * k > d.sms ? (size_t)d.smem_per_sm / 2 : (size_t)d.max_smem_optin) - 4096;
-            const int64_t need = (c.positions / k + t.phases) / t.phases + 1;
-            int64_t keep = fixed < room ? (int64_t)(room - fixed) / iter_bytes : 0;
-            keep = std::min(keep, (need + sum_rows - 1) / sum_rows * sum_rows);
-            t.keep = (int)(keep / sum_rows * sum_rows);
-            p.smem = fixed + (size_t)t.keep * iter_bytes;
-            p.cluster = p.smem + 4096 <= (size_t)d.max_smem_optin;
+            const size_t fixed = need.beside(t.tile, t.phases, (int)(slab / B.d), same);
+            // The blocks that will share an SM, and their room in it.
+            const int share = (int)std::max<int64_t>(
+                1, std::min<int64_t>(need.per_sm, sg::ceil_div(clusters * k, d.sms)));
+            const size_t room = std::min<size_t>(d.smem_per_sm / share - 1024,
+                                                 d.max_smem_optin) - 64;
+            const int per_block = (c.positions + k - 1) / k;
+            const int64_t rows = (per_block + t.phases - 1) / t.phases;
+            const int64_t batches = std::max<int64_t>(1, (rows + need.rows - 1) / need.rows);
+            const int64_t fit = fixed < room ? (int64_t)((room - fixed) / need.batch_bytes) : 0;
+            if (batches <= fit) {  // every row stays; all are asked for at once
+                t.keep = (int)batches;
+                t.ahead = batches > 4 ? 8 : batches > 2 ? 4 : batches > 1 ? 2 : 1;
+                // No ring: its batches are never reached.
+                p.smem = fixed + (size_t)batches * need.batch_bytes;
+                t.keep_all = 1;
+                p.cluster = true;
+            } else if (fit >= 4) {
+                t.ahead = fit >= 12 ? 4 : 2;
+                t.keep = (int)(fit - t.ahead);
+                t.keep_all = 0;
+                p.smem = fixed + (size_t)fit * need.batch_bytes;
+                p.cluster = true;
+            }
             p.grid = (unsigned)(clusters * k);
             if (p.cluster) {
                 t.kept.lanes = lanes;
@@ -1155,9 +1397,12 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
     B.slab = c.channels;
     B.slabs = 1;
     B.keep = 0;
+    B.keep_all = 0;
+    B.ahead = KA;
     // One wave of blocks, eight rows a thread at least.
     const int64_t rows = std::max<int64_t>(1, sg::ceil_div(B.s, 8 * B.phases));
-    B.chunks = (int)std::max<int64_t>(1, std::min(rows, (int64_t)3 * d.sms / std::max(1, B.n)));
+    B.chunks = (int)std::max<int64_t>(
+        1, std::min(rows, (int64_t)need.per_sm * d.sms / std::max(1, B.n)));
     p.grid = (unsigned)B.n * (unsigned)B.chunks;
     return p;
 }
@@ -1230,9 +1475,16 @@ int simtgo_GroupNorm(void* y, float* mean, float* rstd, const void* x, const voi
         c.type, {{x, rx.pitch0 / e, rx.pitch1 / e}, {y, ry.pitch0 / e, ry.pitch1 / e}});
     if (kept && width == 16 && (c.channels % kUnit || ((uintptr_t)codes & 7))) width = 4;
     const bool same = (c.channels / c.groups) % kUnit == 0;
-    const Plan p = make_plan(B, c, *d, kept, e, e == 2 ? 8 : 4, kThreads * kUnit * e,
-                             (int)sizeof(Moments) * (same ? 1 : kUnit),
-                             (int)(sizeof(Moments) + sizeof(float2)));
+    const bool half = c.type != SIMTGO_F32;
+    const int64_t batch_bytes = half ? FwdRow<__half>::kRows * FwdRow<__half>::kBytes * kThreads
+                                     : FwdRow<float>::kRows * FwdRow<float>::kBytes * kThreads;
+    const Needs need = {(double)e, half ? FwdRow<__half>::kRows : FwdRow<float>::kRows, batch_bytes,
+                        [](int tile, int phases, int groups, bool same) {
+                            return 4 * (size_t)cell_floats(phases, tile * (same ? 1 : kUnit), same) +
+                                   groups * (sizeof(Moments) + sizeof(Stat));
+                        },
+                        kBlocks};
+    const Plan p = make_plan(B, c, *d, kept, need);
     cudaStream_t s = (cudaStream_t)stream;
     return by_type(c.type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -1249,8 +1501,9 @@ int simtgo_GroupNorm(void* y, float* mean, float* rstd, const void* x, const voi
             float* own = (float*)(part + parts);
             if (!mean) B.mean_out = own;
             if (!rstd) B.rstd_out = own + stats;
+            const size_t ring = (size_t)B.ahead * batch_bytes;
             const size_t smem =
-                sizeof(Moments) * (S ? 1 : kUnit) * ((size_t)B.units + (size_t)B.phases * B.tile);
+                ring + 4 * (size_t)cell_floats(B.phases, B.tile * (S ? 1 : kUnit), S);
             if (int rc2 = launch<k_stats<T, AW, S>>(*d, p.grid, kThreads, smem, s, 1, false, B,
                                                     part))
                 return rc2;
@@ -1260,7 +1513,7 @@ int simtgo_GroupNorm(void* y, float* mean, float* rstd, const void* x, const voi
                                          (const Moments*)part, wide, blocks))
                 return rc2;
             if (!elems) return 0;
-            return launch<k_apply<T, AW, S, Q>>(*d, p.grid, kThreads, 0, s, 1, true, B);
+            return launch<k_apply<T, AW, S, Q>>(*d, p.grid, kThreads, ring, s, 1, true, B);
         };
         if (same) return kept ? run(std::true_type(), std::true_type())
                               : run(std::true_type(), std::false_type());
@@ -1349,10 +1602,19 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
                                       {dx, rd.pitch0 / e, rd.pitch1 / e}});
     if (from && width == 16 && (c.channels % kUnit || ((uintptr_t)codes & 7))) width = 4;
     const bool same = (c.channels / c.groups) % kUnit == 0;
-    const int unit_bytes = kUnit * e + (from ? 12 : kUnit * e);
-    const Plan p = make_plan(B, c, *d, false, from ? e + 1.1 : 2.0 * e, e == 2 ? 4 : 2,
-                             kThreads * unit_bytes, (int)sizeof(float2) * kUnit,
-                             2 * (int)sizeof(float2));
+    const bool half = c.type != SIMTGO_F32;
+    const int back_rows_ = half ? BackRow<__half, true>::kRows : BackRow<float, true>::kRows;
+    const int64_t batch_bytes =
+        (int64_t)back_rows_ * kThreads *
+        (half ? (from ? BackRow<__half, true>::kBytes : BackRow<__half, false>::kBytes)
+              : (from ? BackRow<float, true>::kBytes : BackRow<float, false>::kBytes));
+    const Needs need = {from ? e + 1.1 : 2.0 * e, back_rows_, batch_bytes,
+                        [](int tile, int phases, int groups, bool) {
+                            return (size_t)channel_bytes(phases, tile * kUnit) +
+                                   groups * 2 * sizeof(float2);
+                        },
+                        kBackBlocks};
+    const Plan p = make_plan(B, c, *d, false, need);
     const bool params = dweight || dbias;
     const int64_t parts = params || !p.cluster ? (int64_t)c.samples * B.chunks * c.channels : 0;
     // A sample's own sums: the parts themselves where it is one chunk.
@@ -1375,7 +1637,8 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
                                                              B.chunks, false, B, part))
                     return r;
             } else {
-                const size_t smem = sizeof(float2) * kUnit * (size_t)B.phases * B.tile;
+                const size_t smem = (size_t)B.ahead * batch_bytes +
+                                    channel_bytes(B.phases, B.tile * kUnit);
                 if (int r = launch<k_back_stats<T, AW, F, S>>(*d, p.grid, kThreads, smem, s, 1,
                                                               false, B, part))
                     return r;
@@ -1396,9 +1659,10 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
                                                 (int)add, (float2*)nullptr, dweight, dbias))
                     return r;
             if (p.cluster || !dx) return 0;
-            return launch<k_back_apply<T, AW, F, S>>(*d, p.grid, kThreads,
-                                                     sizeof(float2) * (size_t)c.groups, s, 1, true,
-                                                     B, (const float2*)tot);
+            const size_t smem =
+                (size_t)B.ahead * batch_bytes + sizeof(float2) * (size_t)c.groups;
+            return launch<k_back_apply<T, AW, F, S>>(*d, p.grid, kThreads, smem, s, 1, true, B,
+                                                     (const float2*)tot);
         };
         if (from) return same ? run(std::true_type(), std::true_type())
                               : run(std::true_type(), std::false_type());
