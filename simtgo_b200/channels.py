@@ -70,13 +70,9 @@ def _same(t, like, name, other):
     if t.shape != like.shape:
         raise _lib.LengthError(_lib.ELENGTH, f"channels: {name} has shape {tuple(t.shape)}, "
                                              f"{other} {tuple(like.shape)}")
-    if t.dtype != like.dtype:
+    if t.dtype is not like.dtype:
         raise TypeError(f"channels: {name} is {t.dtype}, {other} {like.dtype}")
-    _on(t, like, name)
-
-
-def _on(t, like, name):
-    if t.get_device() != like.get_device() or not t.is_cuda:
+    if t.get_device() != like.get_device():   # the CPU is device -1
         raise ValueError(f"channels: {name} is on {t.device}, the call on {like.device}")
 
 
@@ -84,14 +80,15 @@ def _flat(t, like, numel, dtype, name):
     """The address of a contiguous array of numel elements (None: no array)."""
     if t is None:
         return None
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"channels: {name} is {t.dtype}, the kernel takes {dtype}")
     if t.numel() != numel:
         raise _lib.LengthError(_lib.ELENGTH, f"channels: {name} has {t.numel()} elements, the "
                                              f"call takes {numel}")
     if not t.is_contiguous():
         raise TypeError(f"channels: {name} must be contiguous")
-    _on(t, like, name)
+    if t.get_device() != like.get_device():
+        raise ValueError(f"channels: {name} is on {t.device}, the call on {like.device}")
     return t.data_ptr()
 
 
@@ -167,12 +164,19 @@ def _gated_cfg(*v):
     return c, C.byref(c)
 
 
-def _call(fn, dev, stream, args):
-    """Runs fn(*args, stream) on device dev."""
-    if stream is None:
-        stream = torch.cuda.current_stream(dev)
-    sp = getattr(stream, "cuda_stream", stream)
-    if dev == torch.cuda.current_device():
+# torch.cuda.current_device() and current_stream(dev).cuda_stream, without the
+# objects they build: a call on a few rows lasts a few microseconds.
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _call(name, dev, stream, *args):
+    """Runs the library's function on device dev, on the caller's stream or on
+    torch's current one."""
+    sp = _raw_stream(dev) if stream is None else getattr(stream, "cuda_stream", stream)
+    fn = getattr(_lib._lib or _lib.load(), name)
+    if dev == _device():
         rc = fn(*args, sp)
     else:
         with torch.cuda.device(dev):
@@ -224,8 +228,8 @@ def GroupNorm(y, x, weight=None, bias=None, *, groups, eps=1e-5, act="none", thr
         block = ckpt.block
     cfg = _norm_cfg(xs, xr, ys, yr, 0, 0, n, s, c, groups, _type(x, "x"), pt, _act(act), block,
                     threshold, eps)[1]
-    _call(_lib.load().simtgo_GroupNorm, dev, stream,
-          (y.data_ptr(), mu, rs, x.data_ptr(), w, b, ln, codes, scales, cfg))
+    _call("simtgo_GroupNorm", dev, stream, y.data_ptr(), mu, rs, x.data_ptr(), w, b, ln, codes,
+          scales, cfg)
 
 
 def GroupNormBackward(dx, dweight, dbias, dy, x, mean, rstd, weight=None, bias=None, *, groups,
@@ -254,10 +258,10 @@ def GroupNormBackward(dx, dweight, dbias, dy, x, mean, rstd, weight=None, bias=N
         dp = dx.data_ptr()
     cfg = _norm_cfg(xs, xr, ys, yr, ds, dr, n, s, c, groups, _type(dy, "dy"), pt, _act(act), block,
                     threshold, eps)[1]
-    _call(_lib.load().simtgo_GroupNorm_backward, dev, stream,
-          (dp, _flat(dweight, dy, c, torch.float32, "dweight"),
-           _flat(dbias, dy, c, torch.float32, "dbias"), dy.data_ptr(), xp, codes, scales, mu, rs,
-           w, b, ln, cfg))
+    _call("simtgo_GroupNorm_backward", dev, stream, dp,
+          _flat(dweight, dy, c, torch.float32, "dweight"),
+          _flat(dbias, dy, c, torch.float32, "dbias"), dy.data_ptr(), xp, codes, scales, mu, rs,
+          w, b, ln, cfg)
 
 
 def Pack8(ckpt, x, *, stream=None):
@@ -268,9 +272,8 @@ def Pack8(ckpt, x, *, stream=None):
     pitch = _rows(x, "x")
     codes, scales = _kept(ckpt, x, "ckpt")
     c = x.shape[-1]
-    _call(_lib.load().simtgo_Pack8, dev, stream,
-          (codes, scales, x.data_ptr(), _type(x, "x"), x.numel() // c if c else 0, c, pitch,
-           ckpt.block))
+    _call("simtgo_Pack8", dev, stream, codes, scales, x.data_ptr(), _type(x, "x"),
+          x.numel() // c if c else 0, c, pitch, ckpt.block)
 
 
 def Unpack8(x, ckpt, *, stream=None):
@@ -279,9 +282,8 @@ def Unpack8(x, ckpt, *, stream=None):
     pitch = _rows(x, "x")
     codes, scales = _kept(ckpt, x, "ckpt")
     c = x.shape[-1]
-    _call(_lib.load().simtgo_Unpack8, dev, stream,
-          (x.data_ptr(), codes, scales, _type(x, "x"), x.numel() // c if c else 0, c, pitch,
-           ckpt.block))
+    _call("simtgo_Unpack8", dev, stream, x.data_ptr(), codes, scales, _type(x, "x"),
+          x.numel() // c if c else 0, c, pitch, ckpt.block)
 
 
 def Gated(y, a, b=None, *, act="silu", threshold=1.0, a_ckpt=None, b_ckpt=None, stream=None):
@@ -309,8 +311,7 @@ def Gated(y, a, b=None, *, act="silu", threshold=1.0, a_ckpt=None, b_ckpt=None, 
     c = a.shape[-1]
     cfg = _gated_cfg(a.numel() // c if c else 0, ap, bp, yp, 0, 0, c, _type(a, "a"), _act(act),
                      block, threshold, 0)[1]
-    _call(_lib.load().simtgo_Gated, dev, stream,
-          (y.data_ptr(), a.data_ptr(), bd, ac, asc, bc, bsc, cfg))
+    _call("simtgo_Gated", dev, stream, y.data_ptr(), a.data_ptr(), bd, ac, asc, bc, bsc, cfg)
 
 
 def GatedBackward(da, db, dy, a, b=None, *, act="silu", threshold=1.0, stream=None):
@@ -344,8 +345,8 @@ def GatedBackward(da, db, dy, a, b=None, *, act="silu", threshold=1.0, stream=No
     c = dy.shape[-1]
     cfg = _gated_cfg(dy.numel() // c if c else 0, ap, bp, yp, out[0][1], out[1][1], c,
                      _type(dy, "dy"), _act(act), block, threshold, 0)[1]
-    _call(_lib.load().simtgo_Gated_backward, dev, stream,
-          (out[0][0], out[1][0], dy.data_ptr(), ad, bd, ac, asc, bc, bsc, cfg))
+    _call("simtgo_Gated_backward", dev, stream, out[0][0], out[1][0], dy.data_ptr(), ad, bd, ac,
+          asc, bc, bsc, cfg)
 
 
 __all__ = ["Checkpoint", "NewCheckpoint", "GroupNorm", "GroupNormBackward", "Pack8", "Unpack8",

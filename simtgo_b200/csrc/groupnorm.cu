@@ -38,7 +38,7 @@ using namespace chan;
 namespace {
 
 #ifndef KB
-#define KB 3
+#define KB 2
 #endif
 #ifndef BKB
 #define BKB 2
@@ -61,7 +61,7 @@ struct Batch {
     int n, s, c, g, d;
     int units, tile, tiles, phases;  // of a row, or of a slab's row
     int slab, slabs;                 // channels of a cluster's slab, slabs of a sample
-    int chunks;                      // blocks that share a sample's rows
+    int chunks, cluster;             // blocks that share a sample's rows, and that form a cluster
     int keep, ahead;                 // batches of rows that stay in shared memory; in flight
     int keep_all;                    // every batch stays: there is no ring
     int ptype, act;
@@ -85,7 +85,10 @@ __device__ __forceinline__ int phase_rows(const Batch& B, int r0, int r1, int ph
 
 // ---- between blocks and grids --------------------------------------------------
 
-constexpr int kCluster = 8;  // blocks of a cluster, at most
+#ifndef KC
+#define KC 8
+#endif
+constexpr int kCluster = KC;  // blocks of a cluster, at most (past 8 a launch attribute)
 
 __device__ __forceinline__ void cluster_arrive() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -394,7 +397,7 @@ struct Moments {  // the mean is k + off; m2: the sum of squared deviations from
 // Joins (na, a) and (nb, b).
 __device__ __forceinline__ Moments join(float na, Moments a, float nb, Moments b) {
     if (na == 0.0f) return b;
-    const float f = nb / (na + nb), d = nb > 0.0f ? (b.k - a.k) + (b.off - a.off) : 0.0f;
+    const float f = __fdividef(nb, na + nb), d = nb > 0.0f ? (b.k - a.k) + (b.off - a.off) : 0.0f;
     return {a.k, __fmaf_rn(d, f, a.off), __fmaf_rn(d * d, na * f, nb > 0.0f ? a.m2 + b.m2 : a.m2)};
 }
 
@@ -481,32 +484,63 @@ __device__ __forceinline__ void join_groups(const CellSums& sums, int phases, in
     while (lanes > along && groups * lanes > kThreads) lanes /= 2;
     const int lane = threadIdx.x % lanes, lc = lane % along, lp = lane / along;
     const int skip = lanes / along;
+    // Phase p has `each` rows, and one more below `extra`. A phase without rows
+    // has zeros in every cell and counts nothing.
+    const int extra = rows % phases;
+    const float each = (float)(rows / phases);
     for (int base = 0; base < groups; base += kThreads / lanes) {
         const int i = base + threadIdx.x / lanes, g = g_lo + i;
         const bool on = i < groups;
         const int c0 = on ? max(g * d, t0) - t0 : 0, c1 = on ? min(g * d + d, t1) - t0 : 0;
         const float k0 = on ? sums.k[c0] : 0.0f, total = (float)rows * (float)(c1 - c0);
         float a = 0.0f, q = 0.0f;
-        for (int p = lp; p < phases; p += skip) {
-            const float n = (float)max((rows - p + phases - 1) / phases, 0);
-            const int at = p * sums.width;
-            for (int c = c0 + lc; c < c1; c += along)
-                a = __fmaf_rn(n, n > 0.0f ? (sums.k[at + c] - k0) + sums.off[at + c] : 0.0f, a);
+        for (int c = c0 + lc; c < c1; c += along) {
+            const float *k = sums.k + c, *off = sums.off + c;
+#pragma unroll 4
+            for (int p = lp; p < phases; p += skip) {
+                const float n = p < extra ? each + 1.0f : each;
+                a = __fmaf_rn(n, (k[p * sums.width] - k0) + off[p * sums.width], a);
+            }
         }
         for (int o = lanes / 2; o; o /= 2) a += __shfl_xor_sync(~0u, a, o);
-        const float off = total > 0.0f ? a / total : 0.0f;
-        for (int p = lp; p < phases; p += skip) {
-            const float n = (float)max((rows - p + phases - 1) / phases, 0);
-            const int at = p * sums.width;
-            for (int c = c0 + lc; c < c1; c += along)
-                if (n > 0.0f) {
-                    const float dv = (sums.k[at + c] - k0) + (sums.off[at + c] - off);
-                    q += __fmaf_rn(n * (float)per * dv, dv, sums.m2[at + c]);
-                }
+        const float off0 = total > 0.0f ? a / total : 0.0f;
+        for (int c = c0 + lc; c < c1; c += along) {
+            const float *k = sums.k + c, *off = sums.off + c, *m2 = sums.m2 + c;
+#pragma unroll 4
+            for (int p = lp; p < phases; p += skip) {
+                const float n = (float)per * (p < extra ? each + 1.0f : each);
+                const float dv = (k[p * sums.width] - k0) + (off[p * sums.width] - off0);
+                q += __fmaf_rn(n * dv, dv, m2[p * sums.width]);
+            }
         }
         for (int o = lanes / 2; o; o /= 2) q += __shfl_xor_sync(~0u, q, o);
-        if (on && lane == 0) f(g, total * (float)per, Moments{k0, off, q});
+        if (on && lane == 0) f(g, total * (float)per, Moments{k0, off0, q});
     }
+}
+
+// Joins a group's moments over the cluster's blocks, which hold chunks `first`
+// and on of a sample of len rows at the same place `own`: on the first of
+// kCluster neighbouring lanes. Returns the count. Every lane calls it.
+__device__ __forceinline__ float join_cluster(const Batch& B, const Moments* own, bool on, int len,
+                                              int first, Moments& q) {
+    const int k = threadIdx.x % kCluster;
+    float have = 0.0f;
+    if (on && k < B.cluster) {
+        int a, e;
+        chunk_rows(len, B.chunks, first + k, a, e);
+        have = (float)(e - a) * (float)B.d;
+        q = {ld_cluster(&own->k, k), ld_cluster(&own->off, k), ld_cluster(&own->m2, k)};
+    }
+#pragma unroll
+    for (int o = kCluster / 2; o; o /= 2) {
+        const float more = __shfl_down_sync(~0u, have, o, kCluster);
+        const Moments m = {__shfl_down_sync(~0u, q.k, o, kCluster),
+                           __shfl_down_sync(~0u, q.off, o, kCluster),
+                           __shfl_down_sync(~0u, q.m2, o, kCluster)};
+        q = join(have, q, more, m);
+        have += more;
+    }
+    return have;
 }
 
 // ---- a unit's parameters ---------------------------------------------------------
@@ -666,28 +700,17 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_norm(Batch B) {
     __syncthreads();
     join_groups(sums, B.phases, r1 - r0, 0, kSame ? cw / kUnit : cw, kSame ? B.d / kUnit : B.d,
                 kSame ? kUnit : 1, [&](int g, float, Moments m) { own[g] = m; });
-    cluster_arrive();
-    cluster_wait();
+    if (B.chunks > 1) {
+        cluster_arrive();
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
     // A group's blocks on neighbouring lanes, joined pairwise.
     for (int base = 0; base < groups; base += kThreads / kCluster) {
         const int g = base + threadIdx.x / kCluster, k = threadIdx.x % kCluster;
         Moments q = {0.0f, 0.0f, 0.0f};
-        float have = 0.0f;
-        if (g < groups && k < B.chunks) {
-            int a, e;
-            chunk_rows(len, B.chunks, k, a, e);
-            have = (float)(e - a) * (float)B.d;
-            q = {ld_cluster(&own[g].k, k), ld_cluster(&own[g].off, k), ld_cluster(&own[g].m2, k)};
-        }
-#pragma unroll
-        for (int o = kCluster / 2; o; o /= 2) {
-            const float more = __shfl_down_sync(~0u, have, o, kCluster);
-            const Moments m = {__shfl_down_sync(~0u, q.k, o, kCluster),
-                               __shfl_down_sync(~0u, q.off, o, kCluster),
-                               __shfl_down_sync(~0u, q.m2, o, kCluster)};
-            q = join(have, q, more, m);
-            have += more;
-        }
+        const float have = join_cluster(B, own + min(g, groups - 1), g < groups, len, 0, q);
         if (g < groups && k == 0) {
             const float mu = len ? q.k + q.off : 0.0f, var = have > 0.0f ? q.m2 / have : 0.0f;
             const float rs = __fdiv_rn(1.0f, __fsqrt_rn(var + B.eps));
@@ -725,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_stats(Batch B, Moments* p
     const int n = blockIdx.x / B.chunks, k = blockIdx.x % B.chunks;
     int r0, r1;
     chunk_rows(valid_rows(B, n), B.chunks, k, r0, r1);
-    Moments* o = part + ((int64_t)n * B.chunks + k) * B.g;
+    Moments* own = reinterpret_cast<Moments*>(sums_at + cell_floats(B.phases, B.tile * E, kSame));
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
     const int most = (r1 - r0 + B.phases - 1) / B.phases;
     const int cells = kSame ? B.c / kUnit : B.c, d = kSame ? B.d / kUnit : B.d;
@@ -736,7 +759,6 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_stats(Batch B, Moments* p
         if (phase < B.phases)
             sum_rows<T, AW, kSame>(feed, Row(B, n, r0 + phase, unit), cnt, sums, phase, u);
         __syncthreads();
-        if (t == B.tiles - 1) grid_release();
         const int t0 = t * B.tile * E, t1 = min(t0 + B.tile * E, cells), odd = t & 1;
         join_groups(sums, B.phases, r1 - r0, t0, t1, d, kSame ? kUnit : 1,
                     [&](int g, float count, Moments m) {
@@ -748,10 +770,31 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_stats(Batch B, Moments* p
                             carry[odd] = m;
                             carried[odd] = count;
                         } else {
-                            o[g] = m;
+                            own[g] = m;
                         }
                     });
         __syncthreads();
+    }
+    grid_release();
+    // The cluster's blocks joined, each block writing every cluster-th group.
+    const int rank = k % B.cluster, first = k - rank;
+    const int len = valid_rows(B, n);
+    Moments* o = part + ((int64_t)n * (B.chunks / B.cluster) + k / B.cluster) * B.g;
+    if (B.cluster > 1) {
+        cluster_arrive();
+        cluster_wait();
+    }
+    const int share = (B.g - rank + B.cluster - 1) / B.cluster;
+    for (int base = 0; base < share; base += kThreads / kCluster) {
+        const int i = base + threadIdx.x / kCluster, g = rank + i * B.cluster;
+        Moments m = {0.0f, 0.0f, 0.0f};
+        const float have = join_cluster(B, own + min(g, B.g - 1), i < share, len, first, m);
+        if (i < share && threadIdx.x % kCluster == 0) o[g] = m;
+        (void)have;
+    }
+    if (B.cluster > 1) {
+        cluster_arrive();
+        cluster_wait();
     }
 }
 
@@ -765,21 +808,21 @@ __global__ void __launch_bounds__(kJoin)
     grid_wait();
     const int n = blockIdx.x / blocks, g = blockIdx.x % blocks * wide + threadIdx.x % wide;
     const int lane = threadIdx.x / wide, lanes = kJoin / wide;
-    const int len = valid_rows(B, n), per = (len + B.chunks - 1) / B.chunks;
+    const int len = valid_rows(B, n), parts = B.chunks / B.cluster;
+    const int64_t per = (int64_t)((len + B.chunks - 1) / B.chunks) * B.cluster;
     double a = 0.0, q = 0.0, ref = 0.0;
     if (g < B.g) {
-        const Moments* p = part + (int64_t)n * B.chunks * B.g + g;
+        const Moments* p = part + (int64_t)n * parts * B.g + g;
         ref = (double)p[0].k + p[0].off;
-        for (int k = lane; k < B.chunks; k += 4 * lanes) {
+        for (int k = lane; k < parts; k += 4 * lanes) {
             Moments m[4];
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (k + j * lanes < B.chunks) m[j] = p[(int64_t)(k + j * lanes) * B.g];
+                if (k + j * lanes < parts) m[j] = p[(int64_t)(k + j * lanes) * B.g];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int64_t first = (int64_t)(k + j * lanes) * per;
-                const int64_t have = min((int64_t)per, len - first);
-                if (k + j * lanes < B.chunks && have > 0) {
+                const int64_t have = min(per, len - (k + j * lanes) * per);
+                if (k + j * lanes < parts && have > 0) {
                     const double c = (double)have * B.d, dv = ((double)m[j].k - ref) + m[j].off;
                     a += c * dv;
                     q += m[j].m2 + c * dv * dv;
@@ -1080,7 +1123,9 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks) k_back_stats(Batch B, f
     const int n = blockIdx.x / B.chunks, k = blockIdx.x % B.chunks;
     int r0, r1;
     chunk_rows(valid_rows(B, n), B.chunks, k, r0, r1);
-    float2* o = part + ((int64_t)n * B.chunks + k) * B.c;
+    // The cluster's blocks added, each writing every cluster-th run of channels.
+    const int rank = k % B.cluster;
+    float2* o = part + ((int64_t)n * (B.chunks / B.cluster) + k / B.cluster) * B.c;
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
     const int most = (r1 - r0 + B.phases - 1) / B.phases;
     for (int t = 0; t < B.tiles; t++) {
@@ -1091,46 +1136,75 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks) k_back_stats(Batch B, f
         back_sums<T, AW, kFrom, kSame>(B, feed, Row(B, n, r0 + phase, unit), q, sums, phase, u,
                                        cnt);
         const int c0 = t * B.tile * kUnit;
-        for (int i = threadIdx.x; i < min(B.tile * kUnit, B.c - c0); i += kThreads)
-            o[c0 + i] = sums.all[i];
+        if (B.cluster > 1) {
+            cluster_arrive();
+            cluster_wait();
+        }
+        for (int i = rank + threadIdx.x * B.cluster; i < min(B.tile * kUnit, B.c - c0);
+             i += kThreads * B.cluster) {
+            float2 v[kCluster];
+#pragma unroll
+            for (int r = 0; r < kCluster; r++)
+                v[r] = r < B.cluster ? make_float2(ld_cluster(&sums.all[i].x, r),
+                                                   ld_cluster(&sums.all[i].y, r))
+                                     : make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int h = kCluster / 2; h; h /= 2)
+#pragma unroll
+                for (int r = 0; r < h; r++) {
+                    v[r].x += v[r + h].x;
+                    v[r].y += v[r + h].y;
+                }
+            o[c0 + i] = v[0];
+        }
+        if (t == B.tiles - 1) grid_release();
+        if (B.cluster > 1) {
+            cluster_arrive();
+            cluster_wait();
+        }
     }
-    grid_release();
 }
 
-// Adds `rows` rows of part for each of a number of spans, in double: to
-// tot[span][c], and to dbias and dweight where there is one span. A block takes
-// 32 channels of a span, its warps the rows in turn.
-constexpr int kAdd = 1024;
-__global__ void __launch_bounds__(kAdd)
-    k_back_join(const float2* part, int64_t rows, int c, int blocks, float2* tot, float* dw,
-                float* db) {
-    __shared__ double2 sm[kAdd / 32][33];
-    grid_wait();
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int64_t span = blockIdx.x / blocks;
-    const int ch = blockIdx.x % blocks * 32 + lane;
-    const float2* p = part + span * rows * c + ch;
+// Adds `rows` rows of part, in double: channels 32*block and on, a block's warps
+// taking the rows in turn. The first warp ends with the sums.
+template <int kWarps>
+__device__ __forceinline__ double2 add_rows(const float2* part, int64_t rows, int c, int block,
+                                            double2 (*sm)[33]) {
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, ch = block * 32 + lane;
     double2 s = make_double2(0.0, 0.0);
     if (ch < c) {
 #pragma unroll 4
-        for (int64_t r = warp; r < rows; r += kAdd / 32) {
-            const float2 v = p[r * c];
+        for (int64_t r = warp; r < rows; r += kWarps) {
+            const float2 v = part[r * c + ch];
             s.x += v.x;
             s.y += v.y;
         }
     }
     sm[warp][lane] = s;
     __syncthreads();
-    for (int h = kAdd / 64; h; h /= 2) {
+    for (int h = kWarps / 2; h; h /= 2) {
         if (warp < h) {
             sm[warp][lane].x += sm[warp + h][lane].x;
             sm[warp][lane].y += sm[warp + h][lane].y;
         }
         __syncthreads();
     }
+    return sm[warp][lane];
+}
+
+// For each of a number of spans of `rows` rows of part: their sum to
+// tot[span][c], and to dbias and dweight where there is one span.
+constexpr int kAdd = 512;
+__global__ void __launch_bounds__(kAdd)
+    k_back_join(const float2* part, int64_t rows, int c, int blocks, float2* tot, float* dw,
+                float* db) {
+    __shared__ double2 sm[kAdd / 32][33];
+    grid_wait();
+    const int64_t span = blockIdx.x / blocks;
+    const int block = blockIdx.x % blocks, ch = block * 32 + threadIdx.x % 32;
+    const double2 s = add_rows<kAdd / 32>(part + span * rows * c, rows, c, block, sm);
     grid_release();
-    if (warp == 0 && ch < c) {
-        s = sm[0][lane];
+    if (threadIdx.x < 32 && ch < c) {
         if (tot) tot[span * c + ch] = make_float2((float)s.x, (float)s.y);
         if (db) db[ch] = (float)s.x;
         if (dw) dw[ch] = (float)s.y;
@@ -1138,14 +1212,27 @@ __global__ void __launch_bounds__(kAdd)
 }
 
 template <class T, int AW, bool kFrom, bool kSame>
-__global__ void __launch_bounds__(kThreads, kBackBlocks) k_back_apply(Batch B, const float2* tot) {
+__global__ void __launch_bounds__(kThreads, kBackBlocks)
+    k_back_apply(Batch B, const float2* tot, float* dw, float* db) {
     extern __shared__ uint4 dyn[];
     grid_wait();
+    // Blocks past the chunks add the samples' sums for dbias and dweight.
+    const int chunks = B.n * B.chunks;
+    if ((int)blockIdx.x >= chunks) {
+        const int block = blockIdx.x - chunks, ch = block * 32 + threadIdx.x % 32;
+        const double2 s = add_rows<kThreads / 32>(tot, B.n, B.c, block,
+                                                  reinterpret_cast<double2(*)[33]>(dyn));
+        if (threadIdx.x < 32 && ch < B.c) {
+            if (db) db[ch] = (float)s.x;
+            if (dw) dw[ch] = (float)s.y;
+        }
+        return;
+    }
     using Row = BackRow<T, kFrom>;
     float2* means = reinterpret_cast<float2*>(  // of every group, negated
         (char*)dyn + (int64_t)B.ahead * Row::kRows * Row::kBytes * kThreads);
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
-    const int id = gridDim.x - 1 - blockIdx.x, n = id / B.chunks;
+    const int id = chunks - 1 - blockIdx.x, n = id / B.chunks;
     const int len = valid_rows(B, n);
     int r0, r1;
     chunk_rows(len, B.chunks, id % B.chunks, r0, r1);
@@ -1252,6 +1339,18 @@ int allow_smem(const sg::DevInfo& d, size_t bytes) {
     return rc;
 }
 
+// Lets a kernel run as clusters of up to 16 blocks, once per device.
+template <auto Kernel>
+int allow_cluster(const sg::DevInfo& d) {
+    static std::atomic<bool> done[64];
+    if (done[d.device & 63].load(std::memory_order_relaxed)) return 0;
+    const int rc = sg::cuda_status(
+        cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+        "cudaFuncSetAttribute(GroupNorm)");
+    if (!rc) done[d.device & 63].store(true, std::memory_order_relaxed);
+    return rc;
+}
+
 // Launches Kernel, as clusters of `cluster` blocks, and with `after` as soon as
 // the kernel before it releases it (it then waits for that one's end itself).
 template <auto Kernel, class... A>
@@ -1271,6 +1370,8 @@ int launch(const sg::DevInfo& d, unsigned grid, int threads, size_t smem, cudaSt
         at[cfg.numAttrs].val.clusterDim.y = 1;
         at[cfg.numAttrs].val.clusterDim.z = 1;
         cfg.numAttrs++;
+        if (cluster > 8)
+            if (int rc = allow_cluster<Kernel>(d)) return rc;
     }
     if (after) {
         at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1351,14 +1452,18 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
         const double bytes = (double)slab * c.positions * need.elem;
         int k = 1;
         while (k < kCluster && c.positions / (2 * k) >= t.phases &&
-               (clusters * k < 2 * d.sms || bytes / k > 96 * 1024))
+               (2 * k * clusters <= need.per_sm * d.sms || bytes / k > 96 * 1024))
             k *= 2;
-        t.chunks = k;
+        t.chunks = t.cluster = k;
         // A block moves about 36 GB/s; a chunked pass fills the GPU but costs
         // two more launches, about 6 us.
         const double us = bytes * clusters / (std::min<double>(clusters * k, 2 * d.sms) * 36e3);
         const double chunked = bytes * clusters / 6.4e6 + 6.0;
+#ifdef V2ONLY
+        if (0) {
+#else
         if (us <= chunked && clusters * k <= 0x7fffffff) {
+#endif
             const size_t fixed = need.beside(t.tile, t.phases, (int)(slab / B.d), same);
             // The blocks that will share an SM, and their room in it.
             const int share = (int)std::max<int64_t>(
@@ -1399,10 +1504,16 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
     B.keep = 0;
     B.keep_all = 0;
     B.ahead = KA;
-    // One wave of blocks, eight rows a thread at least.
+    // One wave of blocks, eight rows a thread at least, in clusters.
     const int64_t rows = std::max<int64_t>(1, sg::ceil_div(B.s, 8 * B.phases));
-    B.chunks = (int)std::max<int64_t>(
-        1, std::min(rows, (int64_t)need.per_sm * d.sms / std::max(1, B.n)));
+    const int64_t wave = (int64_t)need.per_sm * d.sms / std::max(1, B.n);
+    B.chunks = (int)std::max<int64_t>(1, std::min(rows, wave));
+    B.cluster = 1;
+#ifndef KCS
+#define KCS 1
+#endif
+    while (2 * B.cluster <= std::min(B.chunks, KCS)) B.cluster *= 2;
+    B.chunks -= B.chunks % B.cluster;
     p.grid = (unsigned)B.n * (unsigned)B.chunks;
     return p;
 }
@@ -1494,7 +1605,7 @@ int simtgo_GroupNorm(void* y, float* mean, float* rstd, const void* x, const voi
             if (p.cluster)
                 return launch<k_norm<T, AW, S, Q>>(*d, p.grid, kThreads, p.smem, s, B.chunks, false,
                                                    B);
-            const int64_t parts = stats * B.chunks;
+            const int64_t parts = stats * (B.chunks / B.cluster);
             Scratch scratch;
             if (int rc2 = scratch.alloc(sizeof(Moments) * parts + 8 * stats, s)) return rc2;
             Moments* part = (Moments*)scratch.p;
@@ -1503,11 +1614,15 @@ int simtgo_GroupNorm(void* y, float* mean, float* rstd, const void* x, const voi
             if (!rstd) B.rstd_out = own + stats;
             const size_t ring = (size_t)B.ahead * batch_bytes;
             const size_t smem =
-                ring + 4 * (size_t)cell_floats(B.phases, B.tile * (S ? 1 : kUnit), S);
-            if (int rc2 = launch<k_stats<T, AW, S>>(*d, p.grid, kThreads, smem, s, 1, false, B,
+                ring + 4 * (size_t)cell_floats(B.phases, B.tile * (S ? 1 : kUnit), S) +
+                sizeof(Moments) * (size_t)c.groups;
+            if (int rc2 = launch<k_stats<T, AW, S>>(*d, p.grid, kThreads, smem, s, B.cluster, false, B,
                                                     part))
                 return rc2;
-            const int wide = std::min(32, ceil_pow2(c.groups));
+            // Few enough groups to a block that its threads take every chunk in
+            // one round of four loads.
+            int wide = std::min(32, ceil_pow2(c.groups));
+            while (wide > 1 && 4 * (kJoin / wide) < B.chunks / B.cluster) wide /= 2;
             const int blocks = (c.groups + wide - 1) / wide;
             if (int rc2 = launch<k_join>(*d, (unsigned)c.samples * blocks, kJoin, 0, s, 1, true, B,
                                          (const Moments*)part, wide, blocks))
@@ -1616,9 +1731,10 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
                         kBackBlocks};
     const Plan p = make_plan(B, c, *d, false, need);
     const bool params = dweight || dbias;
-    const int64_t parts = params || !p.cluster ? (int64_t)c.samples * B.chunks * c.channels : 0;
+    const int rows_of = p.cluster ? B.chunks : B.chunks / B.cluster;  // rows of part, a sample
+    const int64_t parts = params || !p.cluster ? (int64_t)c.samples * rows_of * c.channels : 0;
     // A sample's own sums: the parts themselves where it is one chunk.
-    const bool spans = !p.cluster && dx && B.chunks > 1;
+    const bool spans = !p.cluster && dx && rows_of > 1;
     const int64_t tots = spans ? (int64_t)c.samples * c.channels : 0;
     Scratch scratch;
     if (parts && (rc = scratch.alloc(sizeof(float2) * (parts + tots), s))) return rc;
@@ -1639,30 +1755,31 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
             } else {
                 const size_t smem = (size_t)B.ahead * batch_bytes +
                                     channel_bytes(B.phases, B.tile * kUnit);
-                if (int r = launch<k_back_stats<T, AW, F, S>>(*d, p.grid, kThreads, smem, s, 1,
+                if (int r = launch<k_back_stats<T, AW, F, S>>(*d, p.grid, kThreads, smem, s, B.cluster,
                                                               false, B, part))
                     return r;
             }
-            const int64_t all = (int64_t)c.samples * B.chunks;
-            if (spans) {
-                const bool one = c.samples == 1;
+            const bool one = c.samples == 1;
+            if (spans)
                 if (int r = launch<k_back_join>(*d, add * c.samples, kAdd, 0, s, 1, true,
-                                                (const float2*)part, (int64_t)B.chunks, c.channels,
+                                                (const float2*)part, (int64_t)rows_of, c.channels,
                                                 (int)add, tot, one ? dweight : nullptr,
                                                 one ? dbias : nullptr))
                     return r;
+            if (p.cluster || !dx) {
+                if (!params) return 0;
+                return launch<k_back_join>(*d, add, kAdd, 0, s, 1, true, (const float2*)part,
+                                           (int64_t)c.samples * rows_of, c.channels, (int)add,
+                                           (float2*)nullptr, dweight, dbias);
             }
-            if (params && !(spans && c.samples == 1))
-                if (int r = launch<k_back_join>(*d, add, kAdd, 0, s, 1, true,
-                                                (const float2*)(spans ? tot : part),
-                                                spans ? (int64_t)c.samples : all, c.channels,
-                                                (int)add, (float2*)nullptr, dweight, dbias))
-                    return r;
-            if (p.cluster || !dx) return 0;
+            // dbias and dweight that the sums of one sample did not give: added by
+            // blocks of the last launch.
+            const unsigned more = params && !(spans && one) ? add : 0;
             const size_t smem =
-                (size_t)B.ahead * batch_bytes + sizeof(float2) * (size_t)c.groups;
-            return launch<k_back_apply<T, AW, F, S>>(*d, p.grid, kThreads, smem, s, 1, true, B,
-                                                     (const float2*)tot);
+                std::max((size_t)B.ahead * batch_bytes + sizeof(float2) * (size_t)c.groups,
+                         sizeof(double2) * 33 * (kThreads / 32));
+            return launch<k_back_apply<T, AW, F, S>>(*d, p.grid + more, kThreads, smem, s, 1, true,
+                                                     B, (const float2*)tot, dweight, dbias);
         };
         if (from) return same ? run(std::true_type(), std::true_type())
                               : run(std::true_type(), std::false_type());
