@@ -80,6 +80,9 @@ def _flat(t, like, numel, dtype, name):
     """The address of a contiguous array of numel elements (None: no array)."""
     if t is None:
         return None
+    if (t.dtype is dtype and t.numel() == numel and t.is_contiguous()
+            and t.get_device() == like.get_device()):
+        return t.data_ptr()
     if t.dtype is not dtype:
         raise TypeError(f"channels: {name} is {t.dtype}, the kernel takes {dtype}")
     if t.numel() != numel:
@@ -87,9 +90,7 @@ def _flat(t, like, numel, dtype, name):
                                              f"call takes {numel}")
     if not t.is_contiguous():
         raise TypeError(f"channels: {name} must be contiguous")
-    if t.get_device() != like.get_device():
-        raise ValueError(f"channels: {name} is on {t.device}, the call on {like.device}")
-    return t.data_ptr()
+    raise ValueError(f"channels: {name} is on {t.device}, the call on {like.device}")
 
 
 def _kept(k, like, name):
@@ -122,7 +123,10 @@ def _batch(t, name):
 
 def _rows(t, name):
     """The pitch of a tensor's rows, all its axes but the last taken as one."""
-    sh, st = t.shape, t.stride()
+    st = t.stride()
+    if len(st) == 2 and st[1] == 1:
+        return st[0]
+    sh = t.shape
     if not sh:
         raise TypeError(f"channels: {name} has no channels")
     if st[-1] != 1 and sh[-1] > 1:

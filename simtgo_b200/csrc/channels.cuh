@@ -128,15 +128,9 @@ struct V8 {
 
 // The assembler may contract a packed product with the addition after it: where
 // the product's own rounding counts (the checkpoint's codes) it is scalar.
-#ifdef SCALAR2
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(__fmul_rn(a.x,b.x),__fmul_rn(a.y,b.y)); }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(__fadd_rn(a.x,b.x),__fadd_rn(a.y,b.y)); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return make_float2(__fmaf_rn(a.x,b.x,c.x),__fmaf_rn(a.y,b.y,c.y)); }
-#else
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-#endif
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 neg2(float2 v) { return make_float2(-v.x, -v.y); }

@@ -37,17 +37,9 @@ using namespace chan;
 
 namespace {
 
-#ifndef KB
-#define KB 2
-#endif
-#ifndef BKB
-#define BKB 2
-#endif
-#ifndef KA
-#define KA 2
-#endif
 constexpr int kThreads = 256;
-constexpr int kBlocks = KB, kBackBlocks = BKB;  // per SM, at least
+constexpr int kBlocks = 2;  // an SM's registers hold, at least
+constexpr int kAhead = 2;   // batches of a ring, where rows do not stay
 constexpr int64_t kMaxElems = int64_t(1) << 46;
 
 struct Batch {
@@ -61,7 +53,7 @@ struct Batch {
     int n, s, c, g, d;
     int units, tile, tiles, phases;  // of a row, or of a slab's row
     int slab, slabs;                 // channels of a cluster's slab, slabs of a sample
-    int chunks, cluster;             // blocks that share a sample's rows, and that form a cluster
+    int chunks;                      // blocks that share a sample's rows
     int keep, ahead;                 // batches of rows that stay in shared memory; in flight
     int keep_all;                    // every batch stays: there is no ring
     int ptype, act;
@@ -85,10 +77,7 @@ __device__ __forceinline__ int phase_rows(const Batch& B, int r0, int r1, int ph
 
 // ---- between blocks and grids --------------------------------------------------
 
-#ifndef KC
-#define KC 8
-#endif
-constexpr int kCluster = KC;  // blocks of a cluster, at most (past 8 a launch attribute)
+constexpr int kCluster = 8;  // blocks of a cluster, at most
 
 __device__ __forceinline__ void cluster_arrive() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -200,6 +189,20 @@ __device__ __forceinline__ Raw<T> shared_unit(uint32_t src) {
     return r;
 }
 
+// f(j) for the first `live` of a batch's U rows. A whole batch has no conditions
+// in it, so that its rows' instructions interleave.
+template <int U, class F>
+__device__ __forceinline__ void each_row(int live, F&& f) {
+    if (live >= U) {
+#pragma unroll
+        for (int j = 0; j < U; j++) f(j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < U; j++)
+            if (j < live) f(j);
+    }
+}
+
 // What a row gives a thread: forward a unit of x; backward one of dy and one of
 // x, or of its checkpoint.
 template <class T>
@@ -226,11 +229,10 @@ struct FwdRow {
             for (int u = 0; u < U; u++)
                 if (u < live) store_unit<T>(slot + u * kBytes * kThreads, r[u]);
         } else {
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (u < live) copy_unit<T, AW>(slot + u * kBytes * kThreads, x, cnt);
-                x += step;
-            }
+            each_row<U>(live, [&](int u) {
+                copy_unit<T, AW>(slot + u * kBytes * kThreads, x + u * step, cnt);
+            });
+            x += U * step;
         }
     }
 };
@@ -334,54 +336,65 @@ struct BackRow {
 };
 
 // A thread's rows in batches: `most` rows for the block's busiest thread, `mine`
-// for this one.
-template <class Row>
+// for this one. start() asks for the first batches, so that whatever comes
+// between it and down() (or up()) hides their latency.
+template <class Row, int AW>
 struct Feed {
+    Row row;
     uint32_t base;
-    int keep, ahead, batches, mine;
-    __device__ __forceinline__ Feed(const Batch& B, void* smem, int most, int rows)
-        : base(shared_addr(smem) + threadIdx.x * 16),
+    int keep, ahead, batches, mine, next, cnt;
+    __device__ __forceinline__ Feed(const Batch& B, const Row& first, void* smem, int most,
+                                    int rows, int channels)
+        : row(first),
+          base(shared_addr(smem) + threadIdx.x * 16),
           keep(B.keep),
           ahead(B.ahead),
           batches((most + Row::kRows - 1) / Row::kRows),
-          mine(rows) {}
+          mine(rows),
+          cnt(channels) {}
     __device__ __forceinline__ uint32_t slot(int b) const {
         const int at = b < keep ? b : keep + (b & (ahead - 1));
         return base + at * (Row::kRows * Row::kBytes * kThreads);
     }
+    __device__ __forceinline__ void ask_down() {
+        if (next < batches) row.template copy<AW>(slot(next), mine - next * Row::kRows, cnt);
+        copy_commit();
+        next++;
+    }
+    __device__ __forceinline__ void start_down() {
+        next = 0;
+        for (int j = 0; j < ahead; j++) ask_down();
+    }
     // Batch by batch, first to last: f(slot, first row of the batch).
-    template <int AW, class F>
-    __device__ __forceinline__ void forward(Row row, int cnt, F&& f) const {
-        for (int b = 0; b < ahead; b++) {
-            if (b < batches) row.template copy<AW>(slot(b), mine - b * Row::kRows, cnt);
-            copy_commit();
-        }
+    template <class F>
+    __device__ __forceinline__ void down(F&& f) {
         for (int b = 0; b < batches; b++) {
             copy_wait(ahead);
             f(slot(b), b * Row::kRows);
-            if (b + ahead < batches)
-                row.template copy<AW>(slot(b + ahead), mine - (b + ahead) * Row::kRows, cnt);
-            copy_commit();
+            ask_down();
         }
     }
-    // Last to first; the kept batches are not copied again. `row` is the first.
-    template <int AW, class F>
-    __device__ __forceinline__ void backward(Row row, int cnt, F&& f) const {
-        int next = batches - 1;
+    // Last to first; the kept batches are not copied again.
+    __device__ __forceinline__ void ask_up() {
+        if (next >= keep) {
+            row.template copy<AW>(slot(next), mine - next * Row::kRows, cnt);
+            row.move(-2 * Row::kRows);
+            next--;
+        }
+        copy_commit();
+    }
+    __device__ __forceinline__ void start_up(const Row& first) {
+        row = first;
+        next = batches - 1;
         row.move(next * Row::kRows);
-        const auto copy_next = [&]() {
-            if (next >= keep) {
-                row.template copy<AW>(slot(next), mine - next * Row::kRows, cnt);
-                row.move(-2 * Row::kRows);
-                next--;
-            }
-            copy_commit();
-        };
-        for (int j = 0; j < ahead; j++) copy_next();
+        for (int j = 0; j < ahead; j++) ask_up();
+    }
+    template <class F>
+    __device__ __forceinline__ void up(F&& f) {
         for (int b = batches - 1; b >= 0; b--) {
             if (b >= keep) copy_wait(ahead);
             f(slot(b), b * Row::kRows);
-            if (b >= keep) copy_next();
+            if (b >= keep) ask_up();
         }
     }
 };
@@ -418,27 +431,25 @@ __host__ __device__ constexpr int cell_floats(int phases, int cells, bool units)
 
 // Sums this thread's cells down its rows and stores their moments.
 template <class T, int AW, bool kSame>
-__device__ __forceinline__ void sum_rows(const Feed<FwdRow<T>>& feed, const FwdRow<T>& rows,
-                                         int cnt, const CellSums& out, int phase, int u) {
+__device__ __forceinline__ void sum_rows(Feed<FwdRow<T>, AW>& feed, const CellSums& out, int phase,
+                                         int u) {
     constexpr int U = FwdRow<T>::kRows, P = kSame ? 1 : 4;
     float2 k[P] = {}, s1[P] = {}, s2[P] = {};
-    feed.template forward<AW>(rows, cnt, [&](uint32_t slot, int first) {
+    feed.down([&](uint32_t slot, int first) {
         if (first == 0 && feed.mine > 0) {
             const V8 v = unpack(shared_unit<T>(slot));
 #pragma unroll
             for (int i = 0; i < P; i++) k[i] = kSame ? both(v.p[0].x) : v.p[i];
         }
+        each_row<U>(feed.mine - first, [&](int j) {
+            const V8 v = unpack(shared_unit<T>(slot + j * FwdRow<T>::kBytes * kThreads));
 #pragma unroll
-        for (int j = 0; j < U; j++)
-            if (first + j < feed.mine) {
-                const V8 v = unpack(shared_unit<T>(slot + j * FwdRow<T>::kBytes * kThreads));
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 dv = sub2(v.p[i], k[kSame ? 0 : i]);
-                    s1[kSame ? 0 : i] = add2(s1[kSame ? 0 : i], dv);
-                    s2[kSame ? 0 : i] = fma2(dv, dv, s2[kSame ? 0 : i]);
-                }
+            for (int i = 0; i < 4; i++) {
+                const float2 dv = sub2(v.p[i], k[kSame ? 0 : i]);
+                s1[kSame ? 0 : i] = add2(s1[kSame ? 0 : i], dv);
+                s2[kSame ? 0 : i] = fma2(dv, dv, s2[kSame ? 0 : i]);
             }
+        });
     });
     const int at = phase * out.width + u * (kSame ? 1 : 8);
     if constexpr (kSame) {
@@ -518,16 +529,16 @@ __device__ __forceinline__ void join_groups(const CellSums& sums, int phases, in
     }
 }
 
-// Joins a group's moments over the cluster's blocks, which hold chunks `first`
-// and on of a sample of len rows at the same place `own`: on the first of
-// kCluster neighbouring lanes. Returns the count. Every lane calls it.
+// Joins a group's moments over the cluster's blocks, which hold the chunks of a
+// sample of len rows, all at the same place `own`: on the first of kCluster
+// neighbouring lanes. Returns the count. Every lane calls it.
 __device__ __forceinline__ float join_cluster(const Batch& B, const Moments* own, bool on, int len,
-                                              int first, Moments& q) {
+                                              Moments& q) {
     const int k = threadIdx.x % kCluster;
     float have = 0.0f;
-    if (on && k < B.cluster) {
+    if (on && k < B.chunks) {
         int a, e;
-        chunk_rows(len, B.chunks, first + k, a, e);
+        chunk_rows(len, B.chunks, k, a, e);
         have = (float)(e - a) * (float)B.d;
         q = {ld_cluster(&own->k, k), ld_cluster(&own->off, k), ld_cluster(&own->m2, k)};
     }
@@ -626,16 +637,16 @@ __device__ __forceinline__ Affine<kSame> affine(const Batch& B, const V8& w, con
 // first; row0 is the first of the `phase_has` rows of its phase (a thread without
 // a unit has rows too: its lane may write a block's scale).
 template <class T, int AW, bool kSame, bool kKeep>
-__device__ __forceinline__ void apply_rows(const Batch& B, const Feed<FwdRow<T>>& feed,
-                                           const FwdRow<T>& rows, int n, int row0, int phase_has,
-                                           int unit, int cnt, bool on, const Affine<kSame>& q) {
+__device__ __forceinline__ void apply_rows(const Batch& B, Feed<FwdRow<T>, AW>& feed, int n,
+                                           int row0, int phase_has, int unit, int cnt, bool on,
+                                           const Affine<kSame>& q) {
     constexpr int U = FwdRow<T>::kRows, S = FwdRow<T>::kBytes * kThreads;
     const int64_t last = row0 + (int64_t)(feed.batches - 1) * U * B.phases;
     T* y = (T*)B.out + n * B.os + last * B.orow + unit * kUnit;
     const int64_t ystep = B.phases * B.orow;
     KeptAt kept;
     if (kKeep) kept = kept_at(B.kept, (int64_t)n * B.s + last, B.phases, unit);
-    feed.template backward<AW>(rows, cnt, [&](uint32_t slot, int first) {
+    feed.up([&](uint32_t slot, int first) {
         Raw<T> raw[U] = {};
         bool live[U];
 #pragma unroll
@@ -643,21 +654,16 @@ __device__ __forceinline__ void apply_rows(const Batch& B, const Feed<FwdRow<T>>
             live[j] = first + j < phase_has;
             if (kKeep && on && live[j]) raw[j] = shared_unit<T>(slot + j * S);
         }
-        T* to = y;
+        each_row<U>(feed.mine - first, [&](int j) {
+            V8 v = unpack(kKeep ? raw[j] : shared_unit<T>(slot + j * S));
 #pragma unroll
-        for (int j = 0; j < U; j++) {
-            if (on && live[j]) {
-                V8 v = unpack(kKeep ? raw[j] : shared_unit<T>(slot + j * S));
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    v.p[i] = fma2(add2(v.p[i], q.minus[i]), q.scale.p[i], q.bias.p[i]);
-                activate<sizeof(T) == 2>(v, B.act, B.param);
-                Raw<T> o;
-                pack(v, o);
-                st_unit<T, AW>(to, o, cnt);
-            }
-            to += ystep;
-        }
+            for (int i = 0; i < 4; i++)
+                v.p[i] = fma2(add2(v.p[i], q.minus[i]), q.scale.p[i], q.bias.p[i]);
+            activate<sizeof(T) == 2>(v, B.act, B.param);
+            Raw<T> o;
+            pack(v, o);
+            st_unit<T, AW>(y + j * ystep, o, cnt);
+        });
         if (kKeep) {
             keep_units<T, AW, U>(raw, B.kept, kept, live, unit, cnt, on);
             kept.codes -= U * kept.codes_step;
@@ -685,16 +691,18 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_norm(Batch B) {
 
     using Row = FwdRow<T>;
     const int most = (r1 - r0 + B.phases - 1) / B.phases;
-    const Feed<Row> feed(B, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0);
+    const Row rows(B, n, r0 + phase, unit);
+    Feed<Row, AW> feed(B, rows, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0, cnt);
+    feed.start_down();
     const int places = B.keep + (B.keep_all ? 0 : B.ahead);
     float* sums_at = reinterpret_cast<float*>((char*)dyn + (int64_t)places * Row::kRows *
                                                               Row::kBytes * kThreads);
     const CellSums sums(sums_at, B.phases, B.tile * E, kSame);
     Moments* own = reinterpret_cast<Moments*>(sums_at + cell_floats(B.phases, B.tile * E, kSame));
     Stat* stat = reinterpret_cast<Stat*>(own + B.slab / B.d);
-    const Row rows(B, n, r0 + phase, unit);
 
-    if (phase < B.phases) sum_rows<T, AW, kSame>(feed, rows, cnt, sums, phase, u);
+    if (phase < B.phases) sum_rows<T, AW, kSame>(feed, sums, phase, u);
+    feed.start_up(rows);
     const V8 w = ld_params(on ? B.w : nullptr, B.ptype, unit * kUnit, cnt, 1.0f);
     const V8 b = ld_params(on ? B.b : nullptr, B.ptype, unit * kUnit, cnt, 0.0f);
     __syncthreads();
@@ -710,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_norm(Batch B) {
     for (int base = 0; base < groups; base += kThreads / kCluster) {
         const int g = base + threadIdx.x / kCluster, k = threadIdx.x % kCluster;
         Moments q = {0.0f, 0.0f, 0.0f};
-        const float have = join_cluster(B, own + min(g, groups - 1), g < groups, len, 0, q);
+        const float have = join_cluster(B, own + min(g, groups - 1), g < groups, len, q);
         if (g < groups && k == 0) {
             const float mu = len ? q.k + q.off : 0.0f, var = have > 0.0f ? q.m2 / have : 0.0f;
             const float rs = __fdiv_rn(1.0f, __fsqrt_rn(var + B.eps));
@@ -727,8 +735,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_norm(Batch B) {
     const int last = c0 + cw - 1;
     const auto q = affine<kSame>(B, w, b, min(unit * kUnit, last), last,
                                  [&](int g) { return stat[g - g0]; });
-    apply_rows<T, AW, kSame, kKeep>(B, feed, rows, n, r0 + phase, phase_rows(B, r0, r1, phase),
-                                    unit, cnt, on, q);
+    apply_rows<T, AW, kSame, kKeep>(B, feed, n, r0 + phase, phase_rows(B, r0, r1, phase), unit, cnt,
+                                    on, q);
     cluster_wait();
 }
 
@@ -748,17 +756,19 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_stats(Batch B, Moments* p
     const int n = blockIdx.x / B.chunks, k = blockIdx.x % B.chunks;
     int r0, r1;
     chunk_rows(valid_rows(B, n), B.chunks, k, r0, r1);
-    Moments* own = reinterpret_cast<Moments*>(sums_at + cell_floats(B.phases, B.tile * E, kSame));
+    Moments* o = part + ((int64_t)n * B.chunks + k) * B.g;
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
     const int most = (r1 - r0 + B.phases - 1) / B.phases;
     const int cells = kSame ? B.c / kUnit : B.c, d = kSame ? B.d / kUnit : B.d;
     for (int t = 0; t < B.tiles; t++) {
         const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
         const bool on = phase < B.phases && unit < B.units;
-        const Feed<Row> feed(B, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0);
-        if (phase < B.phases)
-            sum_rows<T, AW, kSame>(feed, Row(B, n, r0 + phase, unit), cnt, sums, phase, u);
+        Feed<Row, AW> feed(B, Row(B, n, r0 + phase, unit), dyn, most,
+                           on ? phase_rows(B, r0, r1, phase) : 0, cnt);
+        feed.start_down();
+        if (phase < B.phases) sum_rows<T, AW, kSame>(feed, sums, phase, u);
         __syncthreads();
+        if (t == B.tiles - 1) grid_release();
         const int t0 = t * B.tile * E, t1 = min(t0 + B.tile * E, cells), odd = t & 1;
         join_groups(sums, B.phases, r1 - r0, t0, t1, d, kSame ? kUnit : 1,
                     [&](int g, float count, Moments m) {
@@ -770,31 +780,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_stats(Batch B, Moments* p
                             carry[odd] = m;
                             carried[odd] = count;
                         } else {
-                            own[g] = m;
+                            o[g] = m;
                         }
                     });
         __syncthreads();
-    }
-    grid_release();
-    // The cluster's blocks joined, each block writing every cluster-th group.
-    const int rank = k % B.cluster, first = k - rank;
-    const int len = valid_rows(B, n);
-    Moments* o = part + ((int64_t)n * (B.chunks / B.cluster) + k / B.cluster) * B.g;
-    if (B.cluster > 1) {
-        cluster_arrive();
-        cluster_wait();
-    }
-    const int share = (B.g - rank + B.cluster - 1) / B.cluster;
-    for (int base = 0; base < share; base += kThreads / kCluster) {
-        const int i = base + threadIdx.x / kCluster, g = rank + i * B.cluster;
-        Moments m = {0.0f, 0.0f, 0.0f};
-        const float have = join_cluster(B, own + min(g, B.g - 1), i < share, len, first, m);
-        if (i < share && threadIdx.x % kCluster == 0) o[g] = m;
-        (void)have;
-    }
-    if (B.cluster > 1) {
-        cluster_arrive();
-        cluster_wait();
     }
 }
 
@@ -808,8 +797,8 @@ __global__ void __launch_bounds__(kJoin)
     grid_wait();
     const int n = blockIdx.x / blocks, g = blockIdx.x % blocks * wide + threadIdx.x % wide;
     const int lane = threadIdx.x / wide, lanes = kJoin / wide;
-    const int len = valid_rows(B, n), parts = B.chunks / B.cluster;
-    const int64_t per = (int64_t)((len + B.chunks - 1) / B.chunks) * B.cluster;
+    const int len = valid_rows(B, n), parts = B.chunks;
+    const int64_t per = (len + parts - 1) / parts;
     double a = 0.0, q = 0.0, ref = 0.0;
     if (g < B.g) {
         const Moments* p = part + (int64_t)n * parts * B.g + g;
@@ -854,11 +843,13 @@ __global__ void __launch_bounds__(kJoin)
 template <class T, int AW, bool kSame, bool kKeep>
 __global__ void __launch_bounds__(kThreads, kBlocks) k_apply(Batch B) {
     extern __shared__ uint4 dyn[];
-    grid_wait();
     const int id = gridDim.x - 1 - blockIdx.x, n = id / B.chunks;
     int r0, r1;
     chunk_rows(valid_rows(B, n), B.chunks, id % B.chunks, r0, r1);
-    if (r0 >= r1) return;
+    if (r0 >= r1) {
+        grid_wait();
+        return;
+    }
     using Row = FwdRow<T>;
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
     const int most = (r1 - r0 + B.phases - 1) / B.phases;
@@ -866,14 +857,19 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_apply(Batch B) {
     for (int t = 0; t < B.tiles; t++) {
         const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
         const bool on = phase < B.phases && unit < B.units;
-        const Feed<Row> feed(B, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0);
+        const Row rows(B, n, r0 + phase, unit);
+        Feed<Row, AW> feed(B, rows, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0, cnt);
+        feed.start_up(rows);
         const V8 w = ld_params(on ? B.w : nullptr, B.ptype, unit * kUnit, cnt, 1.0f);
         const V8 b = ld_params(on ? B.b : nullptr, B.ptype, unit * kUnit, cnt, 0.0f);
+        // x and the parameters are the caller's; the statistics are the kernel
+        // before's.
+        if (t == 0) grid_wait();
         const auto q = affine<kSame>(B, w, b, min(unit * kUnit, B.c - 1), B.c - 1, [&](int g) {
             return Stat{mu[g], rs[g]};
         });
-        apply_rows<T, AW, kSame, kKeep>(B, feed, Row(B, n, r0 + phase, unit), n, r0 + phase,
-                                        phase_rows(B, r0, r1, phase), unit, cnt, on, q);
+        apply_rows<T, AW, kSame, kKeep>(B, feed, n, r0 + phase, phase_rows(B, r0, r1, phase), unit,
+                                        cnt, on, q);
     }
 }
 
@@ -937,26 +933,23 @@ __host__ __device__ constexpr int channel_bytes(int phases, int channels) {
 // Sums the thread's rows and then the block's phases into sums.all. Every
 // thread calls it; ends with a barrier.
 template <class T, int AW, bool kFrom, bool kSame>
-__device__ __forceinline__ void back_sums(const Batch& B, const Feed<BackRow<T, kFrom>>& feed,
-                                          const BackRow<T, kFrom>& rows,
+__device__ __forceinline__ void back_sums(const Batch& B, Feed<BackRow<T, kFrom>, AW>& feed,
                                           const BackParams<kSame>& q, const ChannelSums& sums,
-                                          int phase, int u, int cnt) {
+                                          int phase, int u) {
     using Row = BackRow<T, kFrom>;
     const int channels = B.tile * kUnit;
     if (phase < B.phases) {
         float2 a[4] = {}, b[4] = {};
-        feed.template forward<AW>(rows, cnt, [&](uint32_t slot, int first) {
+        feed.down([&](uint32_t slot, int first) {
+            each_row<Row::kRows>(feed.mine - first, [&](int j) {
+                V8 xh, dz;
+                slopes<T, kFrom>(B, q, slot + j * Row::kBytes * kThreads, xh, dz);
 #pragma unroll
-            for (int j = 0; j < Row::kRows; j++)
-                if (first + j < feed.mine) {
-                    V8 xh, dz;
-                    slopes<T, kFrom>(B, q, slot + j * Row::kBytes * kThreads, xh, dz);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        a[i] = add2(a[i], dz.p[i]);
-                        b[i] = fma2(dz.p[i], xh.p[i], b[i]);
-                    }
+                for (int i = 0; i < 4; i++) {
+                    a[i] = add2(a[i], dz.p[i]);
+                    b[i] = fma2(dz.p[i], xh.p[i], b[i]);
                 }
+            });
         });
         const int at = phase * sums.width + u * kUnit;
 #pragma unroll
@@ -1022,8 +1015,7 @@ __device__ __forceinline__ void group_sums(const Batch& B, int c0, int groups, A
 // dx of the feed's rows of this thread's unit, last batch first, from the
 // negated means s1 of dz*w and s2 of dz*w*xh.
 template <class T, int AW, bool kFrom, bool kSame>
-__device__ __forceinline__ void back_rows(const Batch& B, const Feed<BackRow<T, kFrom>>& feed,
-                                          const BackRow<T, kFrom>& rows,
+__device__ __forceinline__ void back_rows(const Batch& B, Feed<BackRow<T, kFrom>, AW>& feed,
                                           const BackParams<kSame>& q, const PerGroup<kSame>& s1,
                                           const PerGroup<kSame>& s2, int n, int row0, int unit,
                                           int cnt) {
@@ -1031,22 +1023,17 @@ __device__ __forceinline__ void back_rows(const Batch& B, const Feed<BackRow<T, 
     const int64_t last = row0 + (int64_t)(feed.batches - 1) * Row::kRows * B.phases;
     T* dx = (T*)B.out + n * B.os + last * B.orow + unit * kUnit;
     const int64_t step = B.phases * B.orow;
-    feed.template backward<AW>(rows, cnt, [&](uint32_t slot, int first) {
-        T* to = dx;
+    feed.up([&](uint32_t slot, int first) {
+        each_row<Row::kRows>(feed.mine - first, [&](int j) {
+            V8 xh, dz;
+            slopes<T, kFrom>(B, q, slot + j * Row::kBytes * kThreads, xh, dz);
 #pragma unroll
-        for (int j = 0; j < Row::kRows; j++) {
-            if (first + j < feed.mine) {
-                V8 xh, dz;
-                slopes<T, kFrom>(B, q, slot + j * Row::kBytes * kThreads, xh, dz);
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    dz.p[i] = mul2(q.rstd[i], fma2(xh.p[i], s2[i], fma2(dz.p[i], q.w.p[i], s1[i])));
-                Raw<T> o;
-                pack(dz, o);
-                st_unit<T, AW>(to, o, cnt);
-            }
-            to += step;
-        }
+            for (int i = 0; i < 4; i++)
+                dz.p[i] = mul2(q.rstd[i], fma2(xh.p[i], s2[i], fma2(dz.p[i], q.w.p[i], s1[i])));
+            Raw<T> o;
+            pack(dz, o);
+            st_unit<T, AW>(dx + j * step, o, cnt);
+        });
         dx -= Row::kRows * step;
     });
 }
@@ -1054,7 +1041,7 @@ __device__ __forceinline__ void back_rows(const Batch& B, const Feed<BackRow<T, 
 // One launch for dx: a cluster per slab of a sample. part, where wanted,
 // receives every block's (A, B) of its channels, for k_back_join.
 template <class T, int AW, bool kFrom, bool kSame>
-__global__ void __launch_bounds__(kThreads, kBackBlocks) k_norm_back(Batch B, float2* part) {
+__global__ void __launch_bounds__(kThreads, kBlocks) k_norm_back(Batch B, float2* part) {
     extern __shared__ uint4 dyn[];
     using Row = BackRow<T, kFrom>;
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
@@ -1073,11 +1060,13 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks) k_norm_back(Batch B, fl
     const int unit = c0 / kUnit + u, cnt = min(kUnit, c0 + cw - unit * kUnit);
     const bool on = phase < B.phases && u * kUnit < cw;
 
-    const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, on);
     const int most = (r1 - r0 + B.phases - 1) / B.phases;
-    const Feed<Row> feed(B, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0);
     const Row rows(B, n, r0 + phase, unit);
-    back_sums<T, AW, kFrom, kSame>(B, feed, rows, q, sums, phase, u, cnt);
+    Feed<Row, AW> feed(B, rows, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0, cnt);
+    feed.start_down();
+    const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, on);
+    back_sums<T, AW, kFrom, kSame>(B, feed, q, sums, phase, u);
+    if (B.out) feed.start_up(rows);
     if (part)
         for (int i = threadIdx.x; i < cw; i += kThreads)
             part[((int64_t)n * B.chunks + rank) * B.c + c0 + i] = sums.all[i];
@@ -1108,14 +1097,14 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks) k_norm_back(Batch B, fl
         const int last = c0 + cw - 1, first = min(unit * kUnit, last);
         const auto s1 = per_group<kSame>(first, last, B.d, [&](int g) { return means[g - g0].x; });
         const auto s2 = per_group<kSame>(first, last, B.d, [&](int g) { return means[g - g0].y; });
-        back_rows<T, AW, kFrom, kSame>(B, feed, rows, q, s1, s2, n, r0 + phase, unit, cnt);
+        back_rows<T, AW, kFrom, kSame>(B, feed, q, s1, s2, n, r0 + phase, unit, cnt);
     }
     cluster_wait();
 }
 
 // Over chunks: (A, B) of every channel of a chunk.
 template <class T, int AW, bool kFrom, bool kSame>
-__global__ void __launch_bounds__(kThreads, kBackBlocks) k_back_stats(Batch B, float2* part) {
+__global__ void __launch_bounds__(kThreads, kBlocks) k_back_stats(Batch B, float2* part) {
     extern __shared__ uint4 dyn[];
     using Row = BackRow<T, kFrom>;
     const ChannelSums sums((char*)dyn + (int64_t)B.ahead * Row::kRows * Row::kBytes * kThreads,
@@ -1123,45 +1112,21 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks) k_back_stats(Batch B, f
     const int n = blockIdx.x / B.chunks, k = blockIdx.x % B.chunks;
     int r0, r1;
     chunk_rows(valid_rows(B, n), B.chunks, k, r0, r1);
-    // The cluster's blocks added, each writing every cluster-th run of channels.
-    const int rank = k % B.cluster;
-    float2* o = part + ((int64_t)n * (B.chunks / B.cluster) + k / B.cluster) * B.c;
+    float2* o = part + ((int64_t)n * B.chunks + k) * B.c;
     const int phase = threadIdx.x / B.tile, u = threadIdx.x % B.tile;
     const int most = (r1 - r0 + B.phases - 1) / B.phases;
     for (int t = 0; t < B.tiles; t++) {
         const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
         const bool on = phase < B.phases && unit < B.units;
-        const Feed<Row> feed(B, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0);
+        Feed<Row, AW> feed(B, Row(B, n, r0 + phase, unit), dyn, most,
+                           on ? phase_rows(B, r0, r1, phase) : 0, cnt);
+        feed.start_down();
         const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, on);
-        back_sums<T, AW, kFrom, kSame>(B, feed, Row(B, n, r0 + phase, unit), q, sums, phase, u,
-                                       cnt);
+        back_sums<T, AW, kFrom, kSame>(B, feed, q, sums, phase, u);
         const int c0 = t * B.tile * kUnit;
-        if (B.cluster > 1) {
-            cluster_arrive();
-            cluster_wait();
-        }
-        for (int i = rank + threadIdx.x * B.cluster; i < min(B.tile * kUnit, B.c - c0);
-             i += kThreads * B.cluster) {
-            float2 v[kCluster];
-#pragma unroll
-            for (int r = 0; r < kCluster; r++)
-                v[r] = r < B.cluster ? make_float2(ld_cluster(&sums.all[i].x, r),
-                                                   ld_cluster(&sums.all[i].y, r))
-                                     : make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int h = kCluster / 2; h; h /= 2)
-#pragma unroll
-                for (int r = 0; r < h; r++) {
-                    v[r].x += v[r + h].x;
-                    v[r].y += v[r + h].y;
-                }
-            o[c0 + i] = v[0];
-        }
         if (t == B.tiles - 1) grid_release();
-        if (B.cluster > 1) {
-            cluster_arrive();
-            cluster_wait();
-        }
+        for (int i = threadIdx.x; i < min(B.tile * kUnit, B.c - c0); i += kThreads)
+            o[c0 + i] = sums.all[i];
     }
 }
 
@@ -1212,14 +1177,14 @@ __global__ void __launch_bounds__(kAdd)
 }
 
 template <class T, int AW, bool kFrom, bool kSame>
-__global__ void __launch_bounds__(kThreads, kBackBlocks)
+__global__ void __launch_bounds__(kThreads, kBlocks)
     k_back_apply(Batch B, const float2* tot, float* dw, float* db) {
     extern __shared__ uint4 dyn[];
-    grid_wait();
     // Blocks past the chunks add the samples' sums for dbias and dweight.
     const int chunks = B.n * B.chunks;
     if ((int)blockIdx.x >= chunks) {
         const int block = blockIdx.x - chunks, ch = block * 32 + threadIdx.x % 32;
+        grid_wait();
         const double2 s = add_rows<kThreads / 32>(tot, B.n, B.c, block,
                                                   reinterpret_cast<double2(*)[33]>(dyn));
         if (threadIdx.x < 32 && ch < B.c) {
@@ -1236,23 +1201,30 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks)
     const int len = valid_rows(B, n);
     int r0, r1;
     chunk_rows(len, B.chunks, id % B.chunks, r0, r1);
-    if (r0 >= r1) return;
-    const float inv = -1.0f / ((float)len * (float)B.d);
-    group_sums(B, 0, B.g, [&](int i) { return tot[(int64_t)n * B.c + i]; },
-               [&](int g, float2 v) { means[g] = make_float2(v.x * inv, v.y * inv); });
-    __syncthreads();
-    if (phase >= B.phases) return;
+    if (r0 >= r1) {
+        grid_wait();
+        return;
+    }
     const int most = (r1 - r0 + B.phases - 1) / B.phases;
     for (int t = 0; t < B.tiles; t++) {
         const int unit = t * B.tile + u, cnt = min(kUnit, B.c - unit * kUnit);
-        if (unit >= B.units) break;
-        const Feed<Row> feed(B, dyn, most, phase_rows(B, r0, r1, phase));
-        const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, true);
+        const bool on = phase < B.phases && unit < B.units;
+        const Row rows(B, n, r0 + phase, unit);
+        Feed<Row, AW> feed(B, rows, dyn, most, on ? phase_rows(B, r0, r1, phase) : 0, cnt);
+        feed.start_up(rows);
+        const BackParams<kSame> q = back_params<kSame>(B, n, unit, cnt, on);
+        if (t == 0) {  // the rest is the caller's; the sums are the kernel before's
+            grid_wait();
+            const float inv = -1.0f / ((float)len * (float)B.d);
+            group_sums(B, 0, B.g, [&](int i) { return tot[(int64_t)n * B.c + i]; },
+                       [&](int g, float2 v) { means[g] = make_float2(v.x * inv, v.y * inv); });
+            __syncthreads();
+        }
+        if (!on) continue;
         const int first = unit * kUnit;
         const auto s1 = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return means[g].x; });
         const auto s2 = per_group<kSame>(first, B.c - 1, B.d, [&](int g) { return means[g].y; });
-        back_rows<T, AW, kFrom, kSame>(B, feed, Row(B, n, r0 + phase, unit), q, s1, s2, n,
-                                       r0 + phase, unit, cnt);
+        back_rows<T, AW, kFrom, kSame>(B, feed, q, s1, s2, n, r0 + phase, unit, cnt);
     }
 }
 
@@ -1339,18 +1311,6 @@ int allow_smem(const sg::DevInfo& d, size_t bytes) {
     return rc;
 }
 
-// Lets a kernel run as clusters of up to 16 blocks, once per device.
-template <auto Kernel>
-int allow_cluster(const sg::DevInfo& d) {
-    static std::atomic<bool> done[64];
-    if (done[d.device & 63].load(std::memory_order_relaxed)) return 0;
-    const int rc = sg::cuda_status(
-        cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
-        "cudaFuncSetAttribute(GroupNorm)");
-    if (!rc) done[d.device & 63].store(true, std::memory_order_relaxed);
-    return rc;
-}
-
 // Launches Kernel, as clusters of `cluster` blocks, and with `after` as soon as
 // the kernel before it releases it (it then waits for that one's end itself).
 template <auto Kernel, class... A>
@@ -1370,8 +1330,6 @@ int launch(const sg::DevInfo& d, unsigned grid, int threads, size_t smem, cudaSt
         at[cfg.numAttrs].val.clusterDim.y = 1;
         at[cfg.numAttrs].val.clusterDim.z = 1;
         cfg.numAttrs++;
-        if (cluster > 8)
-            if (int rc = allow_cluster<Kernel>(d)) return rc;
     }
     if (after) {
         at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1454,16 +1412,15 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
         while (k < kCluster && c.positions / (2 * k) >= t.phases &&
                (2 * k * clusters <= need.per_sm * d.sms || bytes / k > 96 * 1024))
             k *= 2;
-        t.chunks = t.cluster = k;
-        // A block moves about 36 GB/s; a chunked pass fills the GPU but costs
-        // two more launches, about 6 us.
-        const double us = bytes * clusters / (std::min<double>(clusters * k, 2 * d.sms) * 36e3);
-        const double chunked = bytes * clusters / 6.4e6 + 6.0;
-#ifdef V2ONLY
-        if (0) {
-#else
+        t.chunks = k;
+        // A block gets through about 5.4 GB/s of its input; chunks, which fill
+        // the GPU, through 1600 GB/s, after about 5 us more of launches and joins.
+        // Measured both ways (us, clusters and chunks): 8x4096x320 bf16 forward
+        // 20 and 26, backward 31 and 34; 4x16384x512 bf16 forward with its
+        // checkpoint 150 and 57, backward 81 and 75.
+        const double us = bytes * clusters / (std::min<double>(clusters * k, 2 * d.sms) * 5.4e3);
+        const double chunked = bytes * clusters / 1.6e6 + 5.0;
         if (us <= chunked && clusters * k <= 0x7fffffff) {
-#endif
             const size_t fixed = need.beside(t.tile, t.phases, (int)(slab / B.d), same);
             // The blocks that will share an SM, and their room in it.
             const int share = (int)std::max<int64_t>(
@@ -1503,17 +1460,11 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
     B.slabs = 1;
     B.keep = 0;
     B.keep_all = 0;
-    B.ahead = KA;
-    // One wave of blocks, eight rows a thread at least, in clusters.
+    B.ahead = kAhead;
+    // One wave of blocks, eight rows a thread at least.
     const int64_t rows = std::max<int64_t>(1, sg::ceil_div(B.s, 8 * B.phases));
     const int64_t wave = (int64_t)need.per_sm * d.sms / std::max(1, B.n);
     B.chunks = (int)std::max<int64_t>(1, std::min(rows, wave));
-    B.cluster = 1;
-#ifndef KCS
-#define KCS 1
-#endif
-    while (2 * B.cluster <= std::min(B.chunks, KCS)) B.cluster *= 2;
-    B.chunks -= B.chunks % B.cluster;
     p.grid = (unsigned)B.n * (unsigned)B.chunks;
     return p;
 }
@@ -1605,7 +1556,7 @@ int simtgo_GroupNorm(void* y, float* mean, float* rstd, const void* x, const voi
             if (p.cluster)
                 return launch<k_norm<T, AW, S, Q>>(*d, p.grid, kThreads, p.smem, s, B.chunks, false,
                                                    B);
-            const int64_t parts = stats * (B.chunks / B.cluster);
+            const int64_t parts = stats * B.chunks;
             Scratch scratch;
             if (int rc2 = scratch.alloc(sizeof(Moments) * parts + 8 * stats, s)) return rc2;
             Moments* part = (Moments*)scratch.p;
@@ -1614,15 +1565,14 @@ int simtgo_GroupNorm(void* y, float* mean, float* rstd, const void* x, const voi
             if (!rstd) B.rstd_out = own + stats;
             const size_t ring = (size_t)B.ahead * batch_bytes;
             const size_t smem =
-                ring + 4 * (size_t)cell_floats(B.phases, B.tile * (S ? 1 : kUnit), S) +
-                sizeof(Moments) * (size_t)c.groups;
-            if (int rc2 = launch<k_stats<T, AW, S>>(*d, p.grid, kThreads, smem, s, B.cluster, false, B,
+                ring + 4 * (size_t)cell_floats(B.phases, B.tile * (S ? 1 : kUnit), S);
+            if (int rc2 = launch<k_stats<T, AW, S>>(*d, p.grid, kThreads, smem, s, 1, false, B,
                                                     part))
                 return rc2;
             // Few enough groups to a block that its threads take every chunk in
             // one round of four loads.
             int wide = std::min(32, ceil_pow2(c.groups));
-            while (wide > 1 && 4 * (kJoin / wide) < B.chunks / B.cluster) wide /= 2;
+            while (wide > 1 && 4 * (kJoin / wide) < B.chunks) wide /= 2;
             const int blocks = (c.groups + wide - 1) / wide;
             if (int rc2 = launch<k_join>(*d, (unsigned)c.samples * blocks, kJoin, 0, s, 1, true, B,
                                          (const Moments*)part, wide, blocks))
@@ -1728,13 +1678,12 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
                             return (size_t)channel_bytes(phases, tile * kUnit) +
                                    groups * 2 * sizeof(float2);
                         },
-                        kBackBlocks};
+                        kBlocks};
     const Plan p = make_plan(B, c, *d, false, need);
     const bool params = dweight || dbias;
-    const int rows_of = p.cluster ? B.chunks : B.chunks / B.cluster;  // rows of part, a sample
-    const int64_t parts = params || !p.cluster ? (int64_t)c.samples * rows_of * c.channels : 0;
+    const int64_t parts = params || !p.cluster ? (int64_t)c.samples * B.chunks * c.channels : 0;
     // A sample's own sums: the parts themselves where it is one chunk.
-    const bool spans = !p.cluster && dx && rows_of > 1;
+    const bool spans = !p.cluster && dx && B.chunks > 1;
     const int64_t tots = spans ? (int64_t)c.samples * c.channels : 0;
     Scratch scratch;
     if (parts && (rc = scratch.alloc(sizeof(float2) * (parts + tots), s))) return rc;
@@ -1755,21 +1704,21 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
             } else {
                 const size_t smem = (size_t)B.ahead * batch_bytes +
                                     channel_bytes(B.phases, B.tile * kUnit);
-                if (int r = launch<k_back_stats<T, AW, F, S>>(*d, p.grid, kThreads, smem, s, B.cluster,
+                if (int r = launch<k_back_stats<T, AW, F, S>>(*d, p.grid, kThreads, smem, s, 1,
                                                               false, B, part))
                     return r;
             }
             const bool one = c.samples == 1;
             if (spans)
                 if (int r = launch<k_back_join>(*d, add * c.samples, kAdd, 0, s, 1, true,
-                                                (const float2*)part, (int64_t)rows_of, c.channels,
+                                                (const float2*)part, (int64_t)B.chunks, c.channels,
                                                 (int)add, tot, one ? dweight : nullptr,
                                                 one ? dbias : nullptr))
                     return r;
             if (p.cluster || !dx) {
                 if (!params) return 0;
                 return launch<k_back_join>(*d, add, kAdd, 0, s, 1, true, (const float2*)part,
-                                           (int64_t)c.samples * rows_of, c.channels, (int)add,
+                                           (int64_t)c.samples * B.chunks, c.channels, (int)add,
                                            (float2*)nullptr, dweight, dbias);
             }
             // dbias and dweight that the sums of one sample did not give: added by
