@@ -80,14 +80,16 @@ constexpr int64_t kMaxElems = int64_t(1) << 46;  // keeps every byte offset far 
 
 // How units fall on blocks. Rows of units: a tile of `tile` units by `phases`
 // rows at a time, `iters` times down the rows. Where every matrix is contiguous
-// and its rows are whole checkpoint blocks (flat), rows mean nothing: a block
-// takes kThreads consecutive units, `iters` times, and no index needs a division
-// or a product.
+// and there is no checkpoint, or rows are whole blocks of it (flat), rows mean
+// nothing: a block takes kThreads consecutive units, `iters` times, and no index
+// needs a division or a product. The elements past the last whole unit, fewer
+// than eight, are one more unit of the last block.
 struct RowGrid {
     int64_t rows, units_total;
     int channels, units, lanes, tiles, tile, phases, iters;
     int shift;  // log2(units per checkpoint block)
     int nblk;   // checkpoint blocks per row
+    int tail;
     bool flat;
 };
 
@@ -102,8 +104,9 @@ RowGrid row_grid(int64_t rows, int channels, int block, bool contiguous, int sms
     g.shift = 0;
     while (block && (kUnit << g.shift) < block) g.shift++;
     g.nblk = block ? (channels + block - 1) / block : 0;
-    g.flat = contiguous && channels % (block ? block : kUnit) == 0;
-    g.units_total = g.flat ? rows * g.units : 0;
+    g.flat = contiguous && (!block || channels % block == 0);
+    g.units_total = g.flat ? rows * channels / kUnit : 0;
+    g.tail = g.flat ? (int)(rows * channels % kUnit) : 0;
     const int upad = (g.units + g.lanes - 1) / g.lanes * g.lanes;
     g.tiles = (upad + kThreads - 1) / kThreads;
     g.tile = ((upad + g.tiles - 1) / g.tiles + g.lanes - 1) / g.lanes * g.lanes;
@@ -114,14 +117,14 @@ RowGrid row_grid(int64_t rows, int channels, int block, bool contiguous, int sms
     const int64_t groups =
         g.flat ? sg::ceil_div(g.units_total, kThreads) : sg::ceil_div(rows, g.phases) * g.tiles;
     g.iters = (int)std::max<int64_t>(1, std::min<int64_t>(kIters, groups / (sms * 8)));
-    while (groups / g.iters > 0x7ffffff0) g.iters *= 2;
+    while (groups / g.iters > 0x7f000000) g.iters *= 2;  // a grid of blocks
     return g;
 }
 Kept kept(const RowGrid& g, int8_t* codes, float* scales) {
     return {codes, scales, g.channels, g.nblk, g.shift, g.lanes};
 }
 int64_t row_blocks(const RowGrid& g) {
-    if (g.flat) return sg::ceil_div(g.units_total, (int64_t)kThreads * g.iters);
+    if (g.flat) return std::max<int64_t>(1, sg::ceil_div(g.units_total, (int64_t)kThreads * g.iters));
     return sg::ceil_div(g.rows, (int64_t)g.phases * g.iters) * g.tiles;
 }
 
@@ -252,9 +255,30 @@ struct GatedArgs {
     float param;
 };
 
+template <class T, bool kGate>
+__device__ __forceinline__ Raw<T> gated_unit(const GatedArgs& k, const Raw<T>& a, const Raw<T>& b) {
+    V8 v = unpack(a);
+    activate<sizeof(T) == 2>(v, k.act, k.param);
+    if (kGate) {
+        const V8 w = unpack(b);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v.p[i] = mul2(v.p[i], w.p[i]);
+    }
+    Raw<T> r;
+    pack(v, r);
+    return r;
+}
+
 template <class T, int AW, bool kFlat, bool kGate, bool kKeep>
 __global__ void __launch_bounds__(kThreads) k_gated(GatedArgs k, RowGrid g) {
     constexpr int U = sizeof(T) == 2 ? 4 : 2;
+    if (kFlat && !kKeep && g.tail && blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+        const int64_t at = g.units_total * kUnit;
+        const Raw<T> a = ld_unit<T, AW>((const T*)k.a + at, g.tail);
+        Raw<T> b = {};
+        if (kGate) b = ld_unit<T, AW>((const T*)k.b + at, g.tail);
+        st_unit<T, AW>((T*)k.y + at, gated_unit<T, kGate>(k, a, b), g.tail);
+    }
     const Place<kFlat> p(g);
     Walk<const T, kFlat> a((const T*)k.a, k.a_pitch, p), b((const T*)k.b, k.b_pitch, p);
     Walk<T, kFlat> y((T*)k.y, k.y_pitch, p);
@@ -272,18 +296,8 @@ __global__ void __launch_bounds__(kThreads) k_gated(GatedArgs k, RowGrid g) {
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (p.on && live[u]) {
-                V8 v = unpack(ra[u]);
-                activate<sizeof(T) == 2>(v, k.act, k.param);
-                if (kGate) {
-                    const V8 w = unpack(rb[u]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v.p[i] = mul2(v.p[i], w.p[i]);
-                }
-                Raw<T> r;
-                pack(v, r);
-                st_unit<T, AW>(y.ahead(u), r, p.cnt);
-            }
+            if (p.on && live[u])
+                st_unit<T, AW>(y.ahead(u), gated_unit<T, kGate>(k, ra[u], rb[u]), p.cnt);
         if (kKeep) {
             if (k.ka.codes)
                 keep_units<T, AW, U, kFlat>(ra, k.ka, ka.at, live, p.unit, p.cnt, p.on);
@@ -339,9 +353,40 @@ struct Source {
     }
 };
 
+template <class T, int AW, bool kGate>
+__device__ __forceinline__ void gated_back_unit(const GatedBackArgs& k, const V8& a, const V8& b,
+                                                const Raw<T>& dy, T* da, T* db, int cnt) {
+    V8 f, s;
+    activate_slope<sizeof(T) == 2>(a, f, s, k.act, k.param);
+    const V8 d = unpack(dy);
+    Raw<T> r;
+    if (kGate && k.db) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) f.p[i] = mul2(f.p[i], d.p[i]);
+        pack(f, r);
+        st_unit<T, AW>(db, r, cnt);
+    }
+    if (k.da) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            s.p[i] = mul2(s.p[i], kGate ? mul2(d.p[i], b.p[i]) : d.p[i]);
+        pack(s, r);
+        st_unit<T, AW>(da, r, cnt);
+    }
+}
+
 template <class T, int AW, bool kFlat, bool kFrom, bool kGate>
 __global__ void __launch_bounds__(kThreads) k_gated_back(GatedBackArgs k, RowGrid g) {
     constexpr int U = kBackRows<T>;
+    if (kFlat && !kFrom && g.tail && blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+        const int64_t at = g.units_total * kUnit;
+        const Raw<T> a = ld_unit<T, AW>((const T*)k.a + at, g.tail);
+        Raw<T> b = {};
+        if (kGate) b = ld_unit<T, AW>((const T*)k.b + at, g.tail);
+        gated_back_unit<T, AW, kGate>(k, unpack(a), unpack(b),
+                                      ld_unit<T, AW>((const T*)k.dy + at, g.tail), (T*)k.da + at,
+                                      (T*)k.db + at, g.tail);
+    }
     const Place<kFlat> p(g);
     if (!p.on) return;
     using In = Source<T, AW, kFlat, kFrom>;
@@ -360,30 +405,9 @@ __global__ void __launch_bounds__(kThreads) k_gated_back(GatedBackArgs k, RowGri
             }
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (it + u < p.rows) {
-                V8 f, s;
-                activate_slope<sizeof(T) == 2>(a[u].get(), f, s, k.act, k.param);
-                const V8 d = unpack(dy[u]);
-                Raw<T> r;
-                if (kGate && k.db) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) f.p[i] = mul2(f.p[i], d.p[i]);
-                    pack(f, r);
-                    st_unit<T, AW>(ob.ahead(u), r, p.cnt);
-                }
-                if (k.da) {
-                    V8 w = d;
-                    if (kGate) {
-                        const V8 gate = b[u].get();
-#pragma unroll
-                        for (int i = 0; i < 4; i++) w.p[i] = mul2(w.p[i], gate.p[i]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) s.p[i] = mul2(s.p[i], w.p[i]);
-                    pack(s, r);
-                    st_unit<T, AW>(oa.ahead(u), r, p.cnt);
-                }
-            }
+            if (it + u < p.rows)
+                gated_back_unit<T, AW, kGate>(k, a[u].get(), kGate ? b[u].get() : V8{}, dy[u],
+                                              oa.ahead(u), ob.ahead(u), p.cnt);
         y.move(U);
         sa.move(U);
         sb.move(U);
@@ -466,7 +490,7 @@ int simtgo_Pack8(int8_t* codes, float* scales, const void* x, int32_t type, int6
     if ((rc = sg::current_device(&d))) return rc;
     const RowGrid g = row_grid(rows, channels, block, rows == 1 || row_pitch == channels, d->sms);
     const int width =
-        with_codes(access_width(type, {{x, rows > 1 ? row_pitch : 0, 0}}), channels, {codes});
+        with_codes(access_width(type, {{x, g.flat || rows == 1 ? 0 : row_pitch, 0}}), channels, {codes});
     return by_type(type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         const auto kernel = g.flat ? k_pack8<T, decltype(w)::value, true>
@@ -497,7 +521,7 @@ int simtgo_Unpack8(void* x, const int8_t* codes, const float* scales, int32_t ty
     if ((rc = sg::current_device(&d))) return rc;
     const RowGrid g = row_grid(rows, channels, block, rows == 1 || row_pitch == channels, d->sms);
     const int width =
-        with_codes(access_width(type, {{x, rows > 1 ? row_pitch : 0, 0}}), channels, {codes});
+        with_codes(access_width(type, {{x, g.flat || rows == 1 ? 0 : row_pitch, 0}}), channels, {codes});
     return by_type(type, width, [&](auto* t, auto w) {
         using T = std::remove_pointer_t<decltype(t)>;
         const auto kernel = g.flat ? k_unpack8<T, decltype(w)::value, true>
@@ -545,7 +569,7 @@ int simtgo_Gated(void* y, const void* a, const void* b, int8_t* a_codes, float* 
     const bool solid_rows = c.rows == 1 || (c.a_pitch == c.channels && c.y_pitch == c.channels &&
                                             (!b || c.b_pitch == c.channels));
     const RowGrid g = row_grid(c.rows, c.channels, ka || kb ? c.block : 0, solid_rows, d->sms);
-    const int m = c.rows > 1;
+    const int m = c.rows > 1 && !g.flat;
     int width = access_width(c.type, {{y, m * c.y_pitch, 0}, {a, m * c.a_pitch, 0},
                                       {b, m * c.b_pitch, 0}});
     if (ka || kb) width = with_codes(width, c.channels, {a_codes, b_codes});
@@ -611,7 +635,7 @@ int simtgo_Gated_backward(void* da, void* db, const void* dy, const void* a, con
                         (!b || c.b_pitch == c.channels) && (!da || c.da_pitch == c.channels) &&
                         (!db || c.db_pitch == c.channels));
     const RowGrid g = row_grid(c.rows, c.channels, from ? c.block : 0, solid_rows, d->sms);
-    const int m = c.rows > 1;
+    const int m = c.rows > 1 && !g.flat;
     int width = access_width(c.type, {{dy, m * c.y_pitch, 0}, {a, m * c.a_pitch, 0},
                                       {b, m * c.b_pitch, 0}, {da, m * c.da_pitch, 0},
                                       {db, m * c.db_pitch, 0}});

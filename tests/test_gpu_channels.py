@@ -184,6 +184,42 @@ def test_one_parameter_alone_and_outputs_left_out():
     assert same_bits(y2, k.y)
 
 
+# Samples that the shared memory of a cluster does not hold: some rows stay
+# there, the others come again from L2, through a ring. And extents at the
+# limits of a batch, a tile and a thread's rows.
+@pytest.mark.parametrize("shape,dtype", [
+    ((40, 8192, 64, 4), F32), ((24, 16384, 128, 8), BF16), ((33, 9000, 80, 8), F16),
+    ((70, 4097, 72, 9), BF16), ((3, 2049, 2048, 4), BF16), ((2, 513, 2056, 2), F32),
+    ((2000, 3, 16, 2), F32), ((5000, 1, 8, 1), BF16), ((1, 100003, 8, 8), F32)], ids=str)
+def test_samples_larger_than_shared_memory(shape, dtype):
+    k = Case(*shape, dtype, "silu", ragged=True, seed=21)
+    kept = ch.NewCheckpoint(k.x, 64)
+    k.forward(ckpt=kept)
+    k.check_forward()
+    k.backward()
+    k.check_backward()
+    live = torch.cat([torch.arange(k.s, device="cuda") < v for v in k.lens])
+    codes, scales = O.pack(k.clean(k.x).reshape(-1, k.c), 64)
+    assert torch.equal(kept.codes.reshape(-1, k.c)[live], codes[live])
+    assert torch.equal(kept.scales.reshape(live.numel(), -1)[live], scales[live])
+    k.dx.fill_(MARK)
+    k.backward(x=kept)
+    k.check_backward(xv=O.restore(codes, scales, 64).reshape(k.x.shape))
+
+
+@pytest.mark.parametrize("n", [1, 7, 8, 9, 2047, 2048, 2049, 65543])
+def test_gated_lengths_around_whole_units(n):
+    g = gen(31)
+    a, b, dy = (normal(g, 1, n, dtype=BF16) for _ in range(3))
+    y, da, db = (torch.full((1, n + 9), MARK, dtype=BF16, device="cuda") for _ in range(3))
+    ch.Gated(y[:, :n], a, b, act="silu")
+    ch.GatedBackward(da[:, :n], db[:, :n], dy, a, b, act="silu")
+    for got, (want, bound) in zip((y, da, db), gated_bounds(
+            a.to(O.F64), b.to(O.F64), dy.to(O.F64), "silu", BF16)):
+        assert_within("gated", got[:, :n], want, bound)
+        assert (got[:, n:] == MARK).all()
+
+
 # ---- group norm: layouts ------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
