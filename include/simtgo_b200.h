@@ -271,7 +271,9 @@ int simtgo_Histogram_allreduce_fused_overwrite(simtgo_comm* comm, int32_t* bins,
  * the element type at the end; sums run in a fixed order, so equal inputs give
  * equal bits. Written buffers must not overlap any other buffer of the call,
  * nor a row another row of the same buffer (SIMTGO_EALIAS). Configurations are
- * HOST pointers, read before the call returns. */
+ * HOST pointers, read before the call returns. Group norm takes stream-ordered
+ * scratch from the library's pool where it needs any (captured, it belongs to
+ * the graph): make the first call on a device before any stream capture. */
 
 /* Element types. */
 enum { SIMTGO_F32 = 0, SIMTGO_BF16 = 1, SIMTGO_F16 = 2 };

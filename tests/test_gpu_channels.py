@@ -706,3 +706,45 @@ def test_more_than_2_31_elements():
         codes, scales = O.pack(x[row:row + 1], 256)
         assert torch.equal(kept.codes[row:row + 1], codes)
         assert torch.equal(back[row:row + 1], O.restore(codes, scales, 256).float().to(BF16))
+
+
+def test_group_norm_of_more_than_2_31_elements():
+    """A sample whose rows repeat has the statistics of one period, so its last
+    rows have the outputs of the period's."""
+    s, c, times = 4096, 136, 4100
+    k = Case(1, s, c, 17, BF16, "silu", seed=5)
+    k.forward()
+    kept = ch.NewCheckpoint(k.x, 64)
+    ch.Pack8(kept, k.x)
+    x = k.x.repeat(1, times, 1)
+    assert x.numel() > 1 << 31
+    y = torch.empty_like(x)
+    big = ch.NewCheckpoint(x, 64)
+    mean, rstd = torch.empty_like(k.mean), torch.empty_like(k.rstd)
+    ch.GroupNorm(y, x, k.w, k.b, mean=mean, rstd=rstd, ckpt=big, **k.args)
+    assert_within("mean", mean, k.mean.to(O.F64), 1e-6 + 0 * k.mean.to(O.F64))
+    assert_within("rstd", rstd, k.rstd.to(O.F64), 1e-5 * k.rstd.to(O.F64))
+    for part in (y[:, :s], y[:, -s:]):   # the same z to 1e-5, so at most a step apart
+        assert_within("y", part, k.y.to(O.F64), 2.0 ** -7 * k.y.to(O.F64).abs() + 1e-4)
+    for part in (slice(None, s), slice(-s, None)):
+        assert torch.equal(big.codes[:, part], kept.codes)
+        assert torch.equal(big.scales[:, part], kept.scales)
+
+
+def test_capture_of_shapes_not_run_before():
+    """After the device's first call, a graph may hold calls of any shape."""
+    warm = Case(1, 8, 8, 1, F32, "none")
+    warm.forward()
+    warm.backward()
+    a, b = Case(3, 77, 56, 7, F16, "gelu", seed=8), Case(1, 30000, 40, 5, F16, "gelu", seed=9)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for k in (a, b):
+            ch.GroupNorm(k.y, k.x, k.w, k.b, mean=k.mean, rstd=k.rstd, **k.args)
+            ch.GroupNormBackward(k.dx, k.dw, k.db, k.dy, k.x, k.mean, k.rstd, k.w, k.b, **k.args)
+    g.replay()
+    g.replay()
+    torch.cuda.synchronize()
+    for k in (a, b):
+        k.check_forward()
+        k.check_backward()
