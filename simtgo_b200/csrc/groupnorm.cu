@@ -441,17 +441,55 @@ __host__ __device__ constexpr int cell_floats(int phases, int cells, bool units)
     return 3 * phases * (units ? cells | 1 : cells + 4);
 }
 
+// A thread's running sums go to its own places in shared memory every kRun rows:
+// however many rows it has, no float32 sum is of more than a run of rows or of
+// runs, and the errors grow with the square root of either.
+constexpr int kRun = 64;
+__device__ __forceinline__ void add4(float* to, float2 a, float2 b) {
+    float4* p = reinterpret_cast<float4*>(to);
+    const float4 v = *p;
+    *p = make_float4(v.x + a.x, v.y + a.y, v.z + b.x, v.w + b.y);
+}
+
 // Sums this thread's cells down its rows and stores their moments.
 template <class T, int AW, bool kSame>
 __device__ __forceinline__ void sum_rows(Feed<FwdRow<T>, AW>& feed, const CellSums& out, int phase,
                                          int u) {
     constexpr int U = FwdRow<T>::kRows, P = kSame ? 1 : 4;
     float2 k[P] = {}, s1[P] = {}, s2[P] = {};
+    const int at = phase * out.width + u * (kSame ? 1 : 8);
+    const auto flush = [&](bool first) {
+        if constexpr (kSame) {
+            const float a = s1[0].x + s1[0].y, q = s2[0].x + s2[0].y;
+            out.off[at] = first ? a : out.off[at] + a;
+            out.m2[at] = first ? q : out.m2[at] + q;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (first) {
+                    *reinterpret_cast<float4*>(out.off + at + 4 * i) = make_float4(
+                        s1[2 * i].x, s1[2 * i].y, s1[2 * i + 1].x, s1[2 * i + 1].y);
+                    *reinterpret_cast<float4*>(out.m2 + at + 4 * i) = make_float4(
+                        s2[2 * i].x, s2[2 * i].y, s2[2 * i + 1].x, s2[2 * i + 1].y);
+                } else {
+                    add4(out.off + at + 4 * i, s1[2 * i], s1[2 * i + 1]);
+                    add4(out.m2 + at + 4 * i, s2[2 * i], s2[2 * i + 1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < P; i++) s1[i] = s2[i] = both(0.0f);
+    };
+    bool flushed = false;
     feed.down([&](uint32_t slot, int first) {
         if (first == 0 && feed.mine > 0) {
             const V8 v = unpack(shared_unit<T>(slot));
 #pragma unroll
             for (int i = 0; i < P; i++) k[i] = kSame ? both(v.p[0].x) : v.p[i];
+        }
+        if (first && first % kRun == 0) {
+            flush(!flushed);
+            flushed = true;
         }
         each_row<U>(feed.mine - first, [&](int j) {
             const V8 v = unpack(shared_unit<T>(slot + j * FwdRow<T>::kBytes * kThreads));
@@ -463,31 +501,36 @@ __device__ __forceinline__ void sum_rows(Feed<FwdRow<T>, AW>& feed, const CellSu
             }
         });
     });
-    const int at = phase * out.width + u * (kSame ? 1 : 8);
+    // From sums about k to a mean and the squares about it.
+    const float inv = feed.mine > 0 ? 1.0f / (float)(feed.mine * (kSame ? kUnit : 1)) : 0.0f;
     if constexpr (kSame) {
-        const float a = s1[0].x + s1[0].y, q = s2[0].x + s2[0].y;
-        const float m = feed.mine > 0 ? a / (float)(kUnit * feed.mine) : 0.0f;
-        const float m2 = __fmaf_rn(-m, a, q);
+        const float a = s1[0].x + s1[0].y + (flushed ? out.off[at] : 0.0f);
+        const float q = s2[0].x + s2[0].y + (flushed ? out.m2[at] : 0.0f);
+        const float m = a * inv, m2 = __fmaf_rn(-m, a, q);
         out.k[at] = k[0].x;
         out.off[at] = m;
         out.m2[at] = m2 < 0.0f ? 0.0f : m2;
     } else {
-        const float2 inv = both(feed.mine > 0 ? 1.0f / (float)feed.mine : 0.0f);
-        float2 m[4], q[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            m[i] = mul2(s1[i], inv);
-            q[i] = fma2(neg2(m[i]), s1[i], s2[i]);
-            q[i] = make_float2(q[i].x < 0.0f ? 0.0f : q[i].x, q[i].y < 0.0f ? 0.0f : q[i].y);
-        }
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const auto put = [&](float* to, float2 a, float2 b) {
-                *reinterpret_cast<float4*>(to + at + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
-            };
-            put(out.k, k[2 * i], k[2 * i + 1]);
-            put(out.off, m[2 * i], m[2 * i + 1]);
-            put(out.m2, q[2 * i], q[2 * i + 1]);
+            float4* k4 = reinterpret_cast<float4*>(out.k + at + 4 * i);
+            float4* o4 = reinterpret_cast<float4*>(out.off + at + 4 * i);
+            float4* m4 = reinterpret_cast<float4*>(out.m2 + at + 4 * i);
+            float2 a = s1[2 * i], b = s1[2 * i + 1], p = s2[2 * i], q = s2[2 * i + 1];
+            if (flushed) {
+                const float4 v = *o4, w = *m4;
+                a = add2(a, make_float2(v.x, v.y));
+                b = add2(b, make_float2(v.z, v.w));
+                p = add2(p, make_float2(w.x, w.y));
+                q = add2(q, make_float2(w.z, w.w));
+            }
+            const float2 m = mul2(a, both(inv)), n = mul2(b, both(inv));
+            p = fma2(neg2(m), a, p);
+            q = fma2(neg2(n), b, q);
+            *k4 = make_float4(k[2 * i].x, k[2 * i].y, k[2 * i + 1].x, k[2 * i + 1].y);
+            *o4 = make_float4(m.x, m.y, n.x, n.y);
+            *m4 = make_float4(p.x < 0.0f ? 0.0f : p.x, p.y < 0.0f ? 0.0f : p.y,
+                              q.x < 0.0f ? 0.0f : q.x, q.y < 0.0f ? 0.0f : q.y);
         }
     }
 }
@@ -952,7 +995,29 @@ __device__ __forceinline__ void back_sums(const Batch& B, Feed<BackRow<T, kFrom>
     const int channels = B.tile * kUnit;
     if (phase < B.phases) {
         float2 a[4] = {}, b[4] = {};
+        const int at = phase * sums.width + u * kUnit;
+        const auto flush = [&](bool first) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (first) {
+                    *reinterpret_cast<float4*>(sums.a + at + 4 * i) =
+                        make_float4(a[2 * i].x, a[2 * i].y, a[2 * i + 1].x, a[2 * i + 1].y);
+                    *reinterpret_cast<float4*>(sums.b + at + 4 * i) =
+                        make_float4(b[2 * i].x, b[2 * i].y, b[2 * i + 1].x, b[2 * i + 1].y);
+                } else {
+                    add4(sums.a + at + 4 * i, a[2 * i], a[2 * i + 1]);
+                    add4(sums.b + at + 4 * i, b[2 * i], b[2 * i + 1]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) a[i] = b[i] = both(0.0f);
+        };
+        bool flushed = false;
         feed.down([&](uint32_t slot, int first) {
+            if (first && first % kRun == 0) {
+                flush(!flushed);
+                flushed = true;
+            }
             each_row<Row::kRows>(feed.mine - first, [&](int j) {
                 V8 xh, dz;
                 slopes<T, kFrom>(B, q, slot + j * Row::kBytes * kThreads, xh, dz);
@@ -963,14 +1028,7 @@ __device__ __forceinline__ void back_sums(const Batch& B, Feed<BackRow<T, kFrom>
                 }
             });
         });
-        const int at = phase * sums.width + u * kUnit;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            *reinterpret_cast<float4*>(sums.a + at + 4 * i) =
-                make_float4(a[2 * i].x, a[2 * i].y, a[2 * i + 1].x, a[2 * i + 1].y);
-            *reinterpret_cast<float4*>(sums.b + at + 4 * i) =
-                make_float4(b[2 * i].x, b[2 * i].y, b[2 * i + 1].x, b[2 * i + 1].y);
-        }
+        flush(!flushed);
     }
     __syncthreads();
     // Several threads to a channel where there are fewer channels than threads.
