@@ -285,7 +285,9 @@ struct BackRow {
         constexpr int U = kRows;
         const uint32_t cs = kX + threadIdx.x * 8 - threadIdx.x * 16;        // codes' place
         const uint32_t ss = kX + 8 * kThreads + threadIdx.x * 4 - threadIdx.x * 16;
-        if constexpr (AW == 16) {
+        // Asynchronously where a unit is few copies: 4x16384x130 f16 43 us, 59 us
+        // through registers; 4x16384x129 float32 (16 copies a row) 76 and 69.
+        if constexpr (AW == 16 || (AW == 4 && sizeof(T) == 2 && !kFrom)) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const uint32_t to = slot + u * kBytes * kThreads;
