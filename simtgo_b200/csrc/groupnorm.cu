@@ -1368,11 +1368,13 @@ Region batch(const char* K, const char* name, const void* p, const simtgo_group_
     return r;
 }
 
-// Lets a kernel have as much shared memory as a block may, once per device.
+// Lets a kernel have as much shared memory as a block may, once per device: the
+// 48 KB that need no leave hold its static shared memory too, so that any
+// dynamic size may be past them.
 template <auto Kernel>
 int allow_smem(const sg::DevInfo& d, size_t bytes) {
     static std::atomic<bool> done[64];
-    if (bytes <= 48 * 1024 || done[d.device & 63].load(std::memory_order_relaxed)) return 0;
+    if (!bytes || done[d.device & 63].load(std::memory_order_relaxed)) return 0;
     cudaFuncAttributes at;
     int rc = sg::cuda_status(cudaFuncGetAttributes(&at, Kernel), "cudaFuncGetAttributes(GroupNorm)");
     if (!rc)

@@ -1,0 +1,63 @@
+"""Edges of the channels-last operators on the GPU: launches near a default
+limit, outlying first values, far tails, the largest extents and numbers,
+other streams, and captures that come first."""
+import ctypes as C
+import math
+import pathlib
+import subprocess
+import sys
+import textwrap
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import channels_oracle as O  # noqa: E402
+from channels_oracle import assert_within  # noqa: E402
+from simtgo_b200 import channels as ch  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+EPS = 1e-5
+HERE = pathlib.Path(__file__).resolve().parent
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape, dtype=F32):
+    return torch.randn(*shape, device="cuda", generator=g).to(dtype)
+
+
+def fresh_process(code):
+    """Runs code where the library has made no call yet."""
+    head = f"import sys; sys.path[:0] = [{str(HERE)!r}, {str(HERE.parent)!r}]\n"
+    r = subprocess.run([sys.executable, "-c", head + textwrap.dedent(code)], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-4000:]
+
+
+def test_first_calls_whose_shared_memory_is_just_under_the_default():
+    """A block of the sums over chunks has static shared memory beside the
+    dynamic: 1360 channels in groups that are no whole units take 49136 bytes
+    and 32. Every access width, before any call that needs more."""
+    fresh_process("""
+        import torch, channels_oracle as O
+        from channels_oracle import assert_within
+        from simtgo_b200 import channels as ch
+        s = 12000
+        for c, groups in ((1360, 16), (2720, 32)):
+            for dtype, off in ((torch.float32, 0), (torch.bfloat16, 0), (torch.float16, 0),
+                               (torch.float32, 1), (torch.bfloat16, 1), (torch.float16, 1),
+                               (torch.bfloat16, 2), (torch.float16, 2)):
+                g = torch.Generator(device="cuda").manual_seed(c + off)
+                buf = torch.randn(s * c + off, device="cuda", generator=g).to(dtype)
+                x = buf[off:].view(1, s, c)
+                y = torch.empty_like(buf)[off:].view(1, s, c)
+                mean, rstd = torch.empty(2, 1, groups, device="cuda")
+                ch.GroupNorm(y, x, groups=groups, mean=mean, rstd=rstd)
+                want, m, r, bound = O.group_norm(x, None, None, groups, 1e-5, "none", 1.0, [s])
+                assert_within("rstd", rstd, r, 2.0 ** -24 * 16 * r)
+                assert_within("y", y, want, bound)
+        """)
