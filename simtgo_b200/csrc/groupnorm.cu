@@ -1,17 +1,17 @@
 // groupnorm.cu -- group norm with an activation over channels-last batches,
 // forward and backward, with the input kept as an 8-bit checkpoint on request.
 //
-// Mathematics. A thread sums x - K and (x - K)^2, K being the first value it
-// meets: the shift keeps the variance exact to a few ulps however far the mean
-// is from zero, since K is one of the values that are summed. Threads, blocks
-// and chunks of a sample are then joined by counts, means and sums of squared
-// deviations (Chan, Golub and LeVeque's pairwise formula), never by raw
-// squares; a mean stays K plus a small offset until the last join, so
-// differences of means do not cancel. The backward pass needs, for each channel
-// of a sample, A = sum dz and B = sum dz*xh: weighted and summed over a group's
-// channels they give the group's two means in dx, and summed over the samples
-// they are dbias and dweight, so one pass over x and dy serves both. All joins
-// run in a fixed order.
+// Mathematics. A thread sums x - K and (x - K)^2 over short runs of rows, K being
+// the mean of the runs before (at first a value that it meets), and joins the
+// runs: the variance stays exact to a few ulps however far the mean is from zero
+// and whatever the first values are. Threads, blocks and chunks of a sample are
+// then joined by counts, means and sums of squared deviations (Chan, Golub and
+// LeVeque's pairwise formula), never by raw squares; a mean stays K plus a small
+// offset until the last join, so differences of means do not cancel. The backward
+// pass needs, for each channel of a sample, A = sum dz and B = sum dz*xh: weighted
+// and summed over a group's channels they give the group's two means in dx, and
+// summed over the samples they are dbias and dweight, so one pass over x and dy
+// serves both. All joins run in a fixed order.
 //
 // Two ways through the data, both reading it once from HBM:
 //
@@ -443,9 +443,9 @@ __host__ __device__ constexpr int cell_floats(int phases, int cells, bool units)
     return 3 * phases * (units ? cells | 1 : cells + 4);
 }
 
-// A thread's running sums go to its own places in shared memory every kRun rows:
-// however many rows it has, no float32 sum is of more than a run of rows or of
-// runs, and the errors grow with the square root of either.
+// A thread sums its rows in runs of at most kRun, which its own places in shared
+// memory collect: however many rows it has, no float32 sum is of more than a run
+// of rows or of runs, and the errors grow with the square root of either.
 constexpr int kRun = 64;
 __device__ __forceinline__ void add4(float* to, float2 a, float2 b) {
     float4* p = reinterpret_cast<float4*>(to);
@@ -453,46 +453,103 @@ __device__ __forceinline__ void add4(float* to, float2 a, float2 b) {
     *p = make_float4(v.x + a.x, v.y + a.y, v.z + b.x, v.w + b.y);
 }
 
-// Sums this thread's cells down its rows and stores their moments.
+// Sums this thread's cells down its rows and stores their moments: run by run,
+// the first about the first row's value (kSame: the mean of its eight) and each
+// further one about the mean so far. About a value K that lies D from a run's
+// mean, n values' squares hold n D^2 that the run's own moment has not; an
+// outlier for K, kept for all rows, would cancel nearly all of the sum (rstd of
+// 64 channels by 65536 positions 3e-5 off for one first value of 4096). A run is
+// at most three times as long as all rows before it, so that of n D^2 the join
+// keeps a quarter at least.
 template <class T, int AW, bool kSame>
 __device__ __forceinline__ void sum_rows(Feed<FwdRow<T>, AW>& feed, const CellSums& out, int phase,
                                          int u) {
     constexpr int U = FwdRow<T>::kRows, P = kSame ? 1 : 4;
+    constexpr float kPer = kSame ? kUnit : 1;  // values of a row in a cell
     float2 k[P] = {}, s1[P] = {}, s2[P] = {};
     const int at = phase * out.width + u * (kSame ? 1 : 8);
-    const auto flush = [&](bool first) {
+    int before = 0;  // rows of the runs that ended
+    // Ends the run of rows [before, rows): its offset from k and its moment, joined
+    // to those before it. Unless it is the last one, k moves to the mean so far,
+    // and the offset becomes what that rounding left.
+    const auto end_run = [&](int rows, bool last) {
+        const float n = (float)(rows - before);
+        const float inv = rows > before ? 1.0f / (n * kPer) : 0.0f;
+        const float f = before ? n / (float)rows : 1.0f, w = (float)before * kPer * f;
         if constexpr (kSame) {
             const float a = s1[0].x + s1[0].y, q = s2[0].x + s2[0].y;
-            out.off[at] = first ? a : out.off[at] + a;
-            out.m2[at] = first ? q : out.m2[at] + q;
+            float off = a * inv, m2 = __fmaf_rn(-off, a, q);
+            m2 = m2 < 0.0f ? 0.0f : m2;
+            if (before) {
+                const float o = out.off[at], d = off - o;
+                off = __fmaf_rn(d, f, o);
+                m2 = __fmaf_rn(d * d, w, m2 + out.m2[at]);
+            }
+            if (!last) {
+                const float to = k[0].x + off, moved = to - k[0].x;
+                off = (k[0].x - (to - moved)) + (off - moved);
+                k[0] = both(to);
+            } else {
+                out.k[at] = k[0].x;
+            }
+            out.off[at] = off;
+            out.m2[at] = m2;
         } else {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                if (first) {
-                    *reinterpret_cast<float4*>(out.off + at + 4 * i) = make_float4(
-                        s1[2 * i].x, s1[2 * i].y, s1[2 * i + 1].x, s1[2 * i + 1].y);
-                    *reinterpret_cast<float4*>(out.m2 + at + 4 * i) = make_float4(
-                        s2[2 * i].x, s2[2 * i].y, s2[2 * i + 1].x, s2[2 * i + 1].y);
-                } else {
-                    add4(out.off + at + 4 * i, s1[2 * i], s1[2 * i + 1]);
-                    add4(out.m2 + at + 4 * i, s2[2 * i], s2[2 * i + 1]);
+                float4* o4 = reinterpret_cast<float4*>(out.off + at + 4 * i);
+                float4* m4 = reinterpret_cast<float4*>(out.m2 + at + 4 * i);
+                const float4 ob = *o4, mb = *m4;
+                float2 off[2], m2[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float2& kj = k[2 * i + j];
+                    const float2 a = s1[2 * i + j];
+                    off[j] = mul2(a, both(inv));
+                    m2[j] = fma2(neg2(off[j]), a, s2[2 * i + j]);
+                    m2[j].x = m2[j].x < 0.0f ? 0.0f : m2[j].x;
+                    m2[j].y = m2[j].y < 0.0f ? 0.0f : m2[j].y;
+                    if (before) {
+                        const float2 o = j ? make_float2(ob.z, ob.w) : make_float2(ob.x, ob.y);
+                        const float2 m = j ? make_float2(mb.z, mb.w) : make_float2(mb.x, mb.y);
+                        const float2 d = sub2(off[j], o);
+                        off[j] = fma2(d, both(f), o);
+                        m2[j] = fma2(mul2(d, d), both(w), add2(m2[j], m));
+                    }
+                    if (!last) {
+                        const float2 to = add2(kj, off[j]), moved = sub2(to, kj);
+                        off[j] = add2(sub2(kj, sub2(to, moved)), sub2(off[j], moved));
+                        kj = to;
+                    }
                 }
+                if (last)
+                    *reinterpret_cast<float4*>(out.k + at + 4 * i) = make_float4(
+                        k[2 * i].x, k[2 * i].y, k[2 * i + 1].x, k[2 * i + 1].y);
+                *o4 = make_float4(off[0].x, off[0].y, off[1].x, off[1].y);
+                *m4 = make_float4(m2[0].x, m2[0].y, m2[1].x, m2[1].y);
             }
         }
 #pragma unroll
         for (int i = 0; i < P; i++) s1[i] = s2[i] = both(0.0f);
+        before = rows;
     };
-    bool flushed = false;
     feed.down([&](uint32_t slot, int first) {
         if (first == 0 && feed.mine > 0) {
             const V8 v = unpack(shared_unit<T>(slot));
+            if constexpr (kSame) {
+                float2 m = both(0.0f);
 #pragma unroll
-            for (int i = 0; i < P; i++) k[i] = kSame ? both(v.p[0].x) : v.p[i];
+                for (int i = 0; i < 4; i++) m = fma2(v.p[i], both(0.125f), m);
+                k[0] = both(m.x + m.y);
+            } else {
+#pragma unroll
+                for (int i = 0; i < P; i++) k[i] = v.p[i];
+            }
         }
-        if (first && first % kRun == 0) {
-            flush(!flushed);
-            flushed = true;
-        }
+        // A thread that has rows has them all here: at most its last is missing.
+        if (first && feed.mine > 0 &&
+            (first % kRun == 0 || first == U || first == 4 * U || first == 16 * U))
+            end_run(first, false);
         each_row<U>(feed.mine - first, [&](int j) {
             const V8 v = unpack(shared_unit<T>(slot + j * FwdRow<T>::kBytes * kThreads));
 #pragma unroll
@@ -503,38 +560,7 @@ __device__ __forceinline__ void sum_rows(Feed<FwdRow<T>, AW>& feed, const CellSu
             }
         });
     });
-    // From sums about k to a mean and the squares about it.
-    const float inv = feed.mine > 0 ? 1.0f / (float)(feed.mine * (kSame ? kUnit : 1)) : 0.0f;
-    if constexpr (kSame) {
-        const float a = s1[0].x + s1[0].y + (flushed ? out.off[at] : 0.0f);
-        const float q = s2[0].x + s2[0].y + (flushed ? out.m2[at] : 0.0f);
-        const float m = a * inv, m2 = __fmaf_rn(-m, a, q);
-        out.k[at] = k[0].x;
-        out.off[at] = m;
-        out.m2[at] = m2 < 0.0f ? 0.0f : m2;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            float4* k4 = reinterpret_cast<float4*>(out.k + at + 4 * i);
-            float4* o4 = reinterpret_cast<float4*>(out.off + at + 4 * i);
-            float4* m4 = reinterpret_cast<float4*>(out.m2 + at + 4 * i);
-            float2 a = s1[2 * i], b = s1[2 * i + 1], p = s2[2 * i], q = s2[2 * i + 1];
-            if (flushed) {
-                const float4 v = *o4, w = *m4;
-                a = add2(a, make_float2(v.x, v.y));
-                b = add2(b, make_float2(v.z, v.w));
-                p = add2(p, make_float2(w.x, w.y));
-                q = add2(q, make_float2(w.z, w.w));
-            }
-            const float2 m = mul2(a, both(inv)), n = mul2(b, both(inv));
-            p = fma2(neg2(m), a, p);
-            q = fma2(neg2(n), b, q);
-            *k4 = make_float4(k[2 * i].x, k[2 * i].y, k[2 * i + 1].x, k[2 * i + 1].y);
-            *o4 = make_float4(m.x, m.y, n.x, n.y);
-            *m4 = make_float4(p.x < 0.0f ? 0.0f : p.x, p.y < 0.0f ? 0.0f : p.y,
-                              q.x < 0.0f ? 0.0f : q.x, q.y < 0.0f ? 0.0f : q.y);
-        }
-    }
+    end_run(feed.mine, true);
 }
 
 // Joins the cells [t0, t1) that lie in `sums` over all phases into the moments

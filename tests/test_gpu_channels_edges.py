@@ -61,3 +61,39 @@ def test_first_calls_whose_shared_memory_is_just_under_the_default():
                 assert_within("rstd", rstd, r, 2.0 ** -24 * 16 * r)
                 assert_within("y", y, want, bound)
         """)
+
+
+# Cells (units of eight channels, or single channels) of many rows whose first
+# values lie far out: by a sample's single value, by its first row, and by the
+# first rows of every stretch of rows that a block may start at.
+@pytest.mark.parametrize("where", ["value", "row", "click", "every"])
+@pytest.mark.parametrize("shape,far", [
+    ((1, 65536, 1024, 16), 4096.0),    # over chunks, groups of whole units
+    ((1, 65536, 1900, 38), 4096.0),    # over chunks, other groups
+    ((37, 1024, 2048, 1), 3e5),        # clusters
+    ((37, 1024, 2040, 2), 3e5)], ids=str)
+def test_outlying_first_values(shape, far, where):
+    n, s, c, groups = shape
+    d = c // groups
+    x = normal(gen(41), *shape[:3])
+    if where == "value":
+        x[:, 0, ::d] = far
+    elif where == "row":
+        x[:, 0] = far
+    elif where == "click":
+        x[:, :11, ::d] = -far
+    else:
+        x[:, ::s // 512, ::8] += far
+    y = torch.empty_like(x)
+    mean, rstd = torch.empty(2, n, groups, device="cuda")
+    ch.GroupNorm(y, x, groups=groups, mean=mean, rstd=rstd)
+    step = 8   # the oracle's sums, a few samples at a time
+    for lo in range(0, n, step):
+        part = x[lo:lo + step]
+        wm, wr = O.statistics(part, groups, EPS, [s] * part.shape[0])
+        size = part.to(O.F64).abs().amax((1, 2))[:, None]
+        # A run of rows is at most three times as long as what came before it,
+        # so its squares are at most four times what it adds to the sum of
+        # squared deviations; 4 * 8 roundings, halved by the root.
+        assert_within("mean", mean[lo:lo + step], wm, 2.0 ** -24 * (wm.abs() + 8 * size))
+        assert_within("rstd", rstd[lo:lo + step], wr, 2.0 ** -24 * 16 * wr)
