@@ -148,6 +148,19 @@ def _rows(t, name):
     return sh[-1] if pitch is None else pitch
 
 
+def _extent(v, what):
+    """v, an extent that the library takes in 32 bits: ctypes would wrap it."""
+    if v > 0x7fffffff:
+        raise _lib.SimtgoError(_lib.ESIZE, f"channels: {v} {what}, at most {0x7fffffff}")
+    return v
+
+
+def _matrix(t):
+    """(rows, channels) of a tensor of rows."""
+    c = _extent(t.shape[-1], "channels")
+    return t.numel() // c if c else 0, c
+
+
 def _act(act):
     k = ACTS.get(act)
     if k is None:
@@ -197,8 +210,8 @@ def _on_gpu(t, name):
 
 def _norm_args(like, groups, weight, bias, mean, rstd, lengths):
     sh = like.shape
-    n, c = sh[0], sh[-1]
-    s = sh[1] if len(sh) == 3 else sh[1] * sh[2]
+    n, c = _extent(sh[0], "samples"), _extent(sh[-1], "channels")
+    s = _extent(sh[1] if len(sh) == 3 else sh[1] * sh[2], "positions")
     if not isinstance(groups, int) or groups <= 0 or c % groups:
         raise ValueError(f"channels: {c} channels are not a whole number of {groups} groups")
     p = weight if weight is not None else bias
@@ -275,9 +288,9 @@ def Pack8(ckpt, x, *, stream=None):
     dev = _on_gpu(x, "x")
     pitch = _rows(x, "x")
     codes, scales = _kept(ckpt, x, "ckpt")
-    c = x.shape[-1]
-    _call("simtgo_Pack8", dev, stream, codes, scales, x.data_ptr(), _type(x, "x"),
-          x.numel() // c if c else 0, c, pitch, ckpt.block)
+    rows, c = _matrix(x)
+    _call("simtgo_Pack8", dev, stream, codes, scales, x.data_ptr(), _type(x, "x"), rows, c,
+          pitch, ckpt.block)
 
 
 def Unpack8(x, ckpt, *, stream=None):
@@ -285,9 +298,9 @@ def Unpack8(x, ckpt, *, stream=None):
     dev = _on_gpu(x, "x")
     pitch = _rows(x, "x")
     codes, scales = _kept(ckpt, x, "ckpt")
-    c = x.shape[-1]
-    _call("simtgo_Unpack8", dev, stream, x.data_ptr(), codes, scales, _type(x, "x"),
-          x.numel() // c if c else 0, c, pitch, ckpt.block)
+    rows, c = _matrix(x)
+    _call("simtgo_Unpack8", dev, stream, x.data_ptr(), codes, scales, _type(x, "x"), rows, c,
+          pitch, ckpt.block)
 
 
 def Gated(y, a, b=None, *, act="silu", threshold=1.0, a_ckpt=None, b_ckpt=None, stream=None):
@@ -312,9 +325,8 @@ def Gated(y, a, b=None, *, act="silu", threshold=1.0, a_ckpt=None, b_ckpt=None, 
             raise ValueError("channels: both checkpoints have the same block")
         bc, bsc = _kept(b_ckpt, a, "b_ckpt")
         block = b_ckpt.block
-    c = a.shape[-1]
-    cfg = _gated_cfg(a.numel() // c if c else 0, ap, bp, yp, 0, 0, c, _type(a, "a"), _act(act),
-                     block, threshold, 0)[1]
+    rows, c = _matrix(a)
+    cfg = _gated_cfg(rows, ap, bp, yp, 0, 0, c, _type(a, "a"), _act(act), block, threshold, 0)[1]
     _call("simtgo_Gated", dev, stream, y.data_ptr(), a.data_ptr(), bd, ac, asc, bc, bsc, cfg)
 
 
@@ -346,9 +358,9 @@ def GatedBackward(da, db, dy, a, b=None, *, act="silu", threshold=1.0, stream=No
             _same(t, dy, name, "dy")
             out.append((t.data_ptr(), _rows(t, name)))
     (ad, ac, asc, ap), (bd, bc, bsc, bp) = src
-    c = dy.shape[-1]
-    cfg = _gated_cfg(dy.numel() // c if c else 0, ap, bp, yp, out[0][1], out[1][1], c,
-                     _type(dy, "dy"), _act(act), block, threshold, 0)[1]
+    rows, c = _matrix(dy)
+    cfg = _gated_cfg(rows, ap, bp, yp, out[0][1], out[1][1], c, _type(dy, "dy"), _act(act), block,
+                     threshold, 0)[1]
     _call("simtgo_Gated_backward", dev, stream, out[0][0], out[1][0], dy.data_ptr(), ad, bd, ac,
           asc, bc, bsc, cfg)
 
