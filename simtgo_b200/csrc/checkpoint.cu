@@ -105,13 +105,13 @@ RowGrid row_grid(int64_t rows, int channels, int block, bool contiguous, int sms
     RowGrid g;
     g.rows = rows;
     g.channels = channels;
-    g.units = (channels + kUnit - 1) / kUnit;
+    g.units = (int)sg::ceil_div(channels, kUnit);  // in 64 bits: any channels may come
     // Lanes that reduce one block together; a row shorter than a block takes
     // only as many as hold it.
     g.lanes = block ? std::min(block / kUnit, ceil_pow2(std::min(g.units, 32))) : 1;
     g.shift = 0;
     while (block && (kUnit << g.shift) < block) g.shift++;
-    g.nblk = block ? (channels + block - 1) / block : 0;
+    g.nblk = block ? (int)sg::ceil_div(channels, block) : 0;
     g.flat = contiguous && (!block || channels % block == 0);
     g.units_total = g.flat ? rows * channels / kUnit : 0;
     g.tail = g.flat ? (int)(rows * channels % kUnit) : 0;

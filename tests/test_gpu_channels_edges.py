@@ -97,3 +97,24 @@ def test_outlying_first_values(shape, far, where):
         # squared deviations; 4 * 8 roundings, halved by the root.
         assert_within("mean", mean[lo:lo + step], wm, 2.0 ** -24 * (wm.abs() + 8 * size))
         assert_within("rstd", rstd[lo:lo + step], wr, 2.0 ** -24 * 16 * wr)
+
+
+def test_one_row_of_the_most_channels():
+    c = (1 << 31) - 1
+    x = torch.empty(1, c, dtype=F16, device="cuda")
+    x.view(-1)[: 1 << 20].copy_(normal(gen(51), 1 << 20, dtype=F16))
+    for lo in range(1 << 20, c, 1 << 28):
+        x[0, lo:lo + (1 << 28)] = 0.5
+    x[0, -1000:] = normal(gen(52), 1000, dtype=F16)
+    kept = ch.NewCheckpoint(x, 32)
+    back = torch.empty_like(x)
+    ch.Pack8(kept, x)
+    ch.Unpack8(back, kept)
+    for part in (slice(0, 1 << 20), slice((c - 4096) // 32 * 32, c)):
+        codes, scales = O.pack(x[:, part], 32)
+        assert torch.equal(kept.codes[:, part], codes)
+        first = part.start // 32
+        assert torch.equal(kept.scales[:, first:first + scales.shape[1]], scales)
+        assert torch.equal(back[:, part], O.restore(codes, scales, 32).float().to(F16))
+    ch.Gated(back, x, act="none")
+    assert torch.equal(back, x)
