@@ -118,3 +118,23 @@ def test_one_row_of_the_most_channels():
         assert torch.equal(back[:, part], O.restore(codes, scales, 32).float().to(F16))
     ch.Gated(back, x, act="none")
     assert torch.equal(back, x)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+def test_gelu_in_its_negative_tail(dtype):
+    """Held to a relative bound: Phi's fit is within 6e-6, exp2's argument of
+    at most 104 carries two roundings (9e-6), the rest a few 2^-23; float32: the
+    argument of erfc carries two roundings, which it multiplies by z^2 + 1, and
+    erfc and the products a few more."""
+    z = -torch.linspace(3, 12, 4001, device="cuda", dtype=O.F64).to(dtype)[None]
+    y, da, one = torch.empty_like(z), torch.empty_like(z), torch.ones_like(z)
+    ch.Gated(y, z, act="gelu")
+    ch.GatedBackward(da, None, one, z, act="gelu")
+    v = z.to(O.F64)
+    rel = 2.0 ** -15 if dtype != F32 else 2.0 ** -23 * (v * v + 9)
+    u = O.HALF_STEP[dtype]
+    want = O.act(v, "gelu")
+    assert_within("gelu", y, want, (u + rel) * want.abs() + O.TINY[dtype])
+    # The slope is Phi - |z| phi: at most 1.3 times its size in each.
+    slope = O.dact(v, "gelu")
+    assert_within("slope", da, slope, (u + 2 * rel) * slope.abs() + O.TINY[dtype])
