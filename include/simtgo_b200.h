@@ -333,8 +333,9 @@ int simtgo_GroupNorm_backward(void* dx, float* dweight, float* dbias, const void
 /* An 8-bit checkpoint of a matrix of `rows` rows, row_pitch elements apart.
  * Each block of `block` consecutive channels of a row (the last one may be
  * shorter) has a = max(largest magnitude, 2^-100), scale = a/127 and codes
- * rint(x * (127/a)), every step rounded to float32, ties to even. A block with
- * a NaN or an infinity gets scale NaN. codes is rows*channels bytes, scales
+ * rint(x * (127/a)), every step rounded to float32, ties to even (the scale of
+ * the largest float down, so that it restores to a finite one). A block with a
+ * NaN or an infinity gets scale NaN. codes is rows*channels bytes, scales
  * rows*ceil(channels/block) floats, both contiguous. */
 int simtgo_Pack8(int8_t* codes, float* scales, const void* x, int32_t type, int64_t rows,
                  int32_t channels, int64_t row_pitch, int32_t block, void* stream);

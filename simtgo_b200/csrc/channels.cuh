@@ -356,8 +356,9 @@ __device__ __forceinline__ void activate_slope(const V8& z, V8& f, V8& d, int ac
 // ---- the 8-bit checkpoint ---------------------------------------------------------
 // A block of `block` consecutive channels of a row shares a float32 scale:
 // a = max(largest magnitude, 2^-100), scale = a/127, code = rint(x * (127/a)),
-// each step rounded to float32. The floor keeps 127/a finite and makes an
-// all-zero block need no case of its own. Magnitudes are compared as bit
+// each step rounded to float32 (the largest float's scale down, so that 127 of it
+// are finite). The floor keeps 127/a finite and makes an all-zero block need no
+// case of its own. Magnitudes are compared as bit
 // patterns, where NaN is above infinity: a block that holds either gets
 // scale NaN, so it restores to NaN throughout and nothing is hidden.
 
@@ -439,7 +440,7 @@ __device__ __forceinline__ void block_scale(uint32_t m, float& scale, float& inv
         return;
     }
     const float a = fmaxf(__uint_as_float(m), 0x1p-100f);
-    scale = __fdiv_rn(a, 127.0f);
+    scale = fminf(__fdiv_rn(a, 127.0f), 0x1.02040600p+121f);  // FLT_MAX/127, rounded down
     inverse = __fdiv_rn(127.0f, a);
 }
 

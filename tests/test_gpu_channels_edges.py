@@ -138,3 +138,19 @@ def test_gelu_in_its_negative_tail(dtype):
     # The slope is Phi - |z| phi: at most 1.3 times its size in each.
     slope = O.dact(v, "gelu")
     assert_within("slope", da, slope, (u + 2 * rel) * slope.abs() + O.TINY[dtype])
+
+
+def test_the_largest_number_restores_to_a_finite_one():
+    top = torch.finfo(F32).max
+    x = torch.zeros(3, 64, device="cuda")
+    x[0, 3], x[1, 40], x[2] = top, -top, top
+    x[0, 4] = top / 2
+    for block in ch.BLOCKS:
+        kept = ch.NewCheckpoint(x, block)
+        back = torch.empty_like(x)
+        ch.Pack8(kept, x)
+        ch.Unpack8(back, kept)
+        assert torch.isfinite(back).all()
+        step = kept.scales.repeat_interleave(block, 1)[:, :64].to(O.F64)
+        assert_within("restored", back, x.to(O.F64), step * 0.50002)
+        assert kept.codes[0, 3] == 127 and kept.codes[1, 40] == -127 and (kept.codes[2] == 127).all()
