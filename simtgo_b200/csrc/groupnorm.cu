@@ -1515,10 +1515,14 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
         t.chunks = k;
         // A block gets through about 5.4 GB/s of its input; chunks, which fill
         // the GPU, through 1600 GB/s, after about 5 us more of launches and joins.
+        // Clusters that fill it reach the same rate, and keep a call up to 8 GB.
         // Measured both ways (us, clusters and chunks): 8x4096x320 bf16 forward
         // 20 and 26, backward 31 and 34; 4x16384x512 bf16 forward with its
-        // checkpoint 150 and 57, backward 81 and 75.
-        const double us = bytes * clusters / (std::min<double>(clusters * k, 2 * d.sms) * 5.4e3);
+        // checkpoint 150 and 57, backward 81 and 75; 600x1000x96 bf16 forward 86
+        // and 104, backward 180 and 151; 64x4096x1024 float32 forward 989 and 851;
+        // above the limit 256x16384x1024 bf16 forward 4791 and 4364, backward 8295
+        // and 8033, 130x16384x1024 float32 without an activation 6031 and 6892.
+        const double us = bytes * clusters / (std::min<double>(clusters * k, need.per_sm * d.sms) * 5.4e3);
         const double chunked = bytes * clusters / 1.6e6 + 5.0;
         if (us <= chunked && clusters * k <= 0x7fffffff) {
             const size_t fixed = need.beside(t.tile, t.phases, (int)(slab / B.d), same);
