@@ -617,18 +617,22 @@ int by_type(int32_t type, int width, F&& f) {
 }
 
 // A buffer of rows: `width` bytes at each combination of up to two pitches
-// (bytes; 0 where it is taken once only), `bytes` from its first to its last.
+// (bytes; 0 where it is taken once only), each taken so many times; `bytes` from
+// its first to its last.
 struct Region {
     const char* name;
     const void* p;
     int64_t width, pitch0, pitch1, bytes;
     bool written;
+    int64_t times0, times1;
 };
 inline Region solid(const char* name, const void* p, int64_t bytes, bool written) {
-    return {name, p, bytes, 0, 0, bytes, written};
+    return {name, p, bytes, 0, 0, bytes, written, 1, 1};
 }
-// SIMTGO_EALIAS for two regions that may overlap, one of them written. Rows of
-// one buffer that interleave (channel slices of the same batch) do not: with
+// SIMTGO_EALIAS for two regions that may overlap, one of them written. Parts of
+// one buffer (channel slices, crops of positions, every second sample of the same
+// batch) do not where none of their rows meet: exactly, where both have the same
+// pitches and counts and one pitch steps over all of the other's rows. Else, with
 // all pitches multiples of P, a region lies in one stretch of the residues mod
 // P, and two such stretches are compared.
 int check_regions(const char* K, std::initializer_list<Region> regions);

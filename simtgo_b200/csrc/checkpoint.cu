@@ -51,6 +51,44 @@ int check_aligned(const char* K, const char* name, const void* p, int bytes) {
     return 0;
 }
 
+// Largest whole number not above a/b, for b > 0.
+static int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+
+// Whether a row of b, `off` bytes on, meets one of a, for regions of the same
+// pitches and counts: rows i, j and i', j' meet where off + (i'-i) in + (j'-j) out
+// lies in (-width, width), and `out` steps over a stretch of all `in` steps, so few
+// differences come near zero.
+static bool rows_meet(const Region& a, const Region& b, int64_t off) {
+    const bool swap = a.pitch0 > a.pitch1;
+    const int64_t in = swap ? a.pitch1 : a.pitch0, n_in = swap ? a.times1 : a.times0;
+    const int64_t out = swap ? a.pitch0 : a.pitch1, n_out = swap ? a.times0 : a.times1;
+    const int64_t j0 = out ? floor_div(-off, out) : 0;
+    for (int64_t j = j0 - 1; j <= j0 + 2; j++) {
+        if (j <= -n_out || j >= n_out) continue;
+        const int64_t at = off + j * out, i0 = in ? floor_div(-at, in) : 0;
+        for (int64_t i = i0; i <= i0 + 1; i++) {
+            const int64_t k = std::max(1 - n_in, std::min(i, n_in - 1)), d = at + k * in;
+            if (d > -b.width && d < a.width) return true;
+        }
+    }
+    return false;
+}
+
+static bool may_meet(const Region& a, const Region& b) {
+    const int64_t off = (int64_t)((uintptr_t)b.p - (uintptr_t)a.p);
+    const int64_t in = std::min(a.pitch0, a.pitch1), out = std::max(a.pitch0, a.pitch1);
+    const int64_t n_in = a.pitch0 > a.pitch1 ? a.times1 : a.times0;
+    if (a.pitch0 == b.pitch0 && a.pitch1 == b.pitch1 && a.times0 == b.times0 &&
+        a.times1 == b.times1 && (out == 0 || out >= (n_in - 1) * in + std::max(a.width, b.width)))
+        return rows_meet(a, b, off);
+    const int64_t period =
+        std::gcd(std::gcd(a.pitch0, a.pitch1), std::gcd(b.pitch0, b.pitch1));
+    if (period <= 0) return true;
+    int64_t r = off % period;
+    if (r < 0) r += period;
+    return r < a.width || r + b.width > period;
+}
+
 int check_regions(const char* K, std::initializer_list<Region> regions) {
     for (const Region* a = regions.begin(); a != regions.end(); a++) {
         if (!a->p || a->bytes <= 0) continue;
@@ -58,13 +96,7 @@ int check_regions(const char* K, std::initializer_list<Region> regions) {
             if (!b->p || b->bytes <= 0 || (!a->written && !b->written)) continue;
             const uintptr_t pa = (uintptr_t)a->p, pb = (uintptr_t)b->p;
             if (pa >= pb + (uintptr_t)b->bytes || pb >= pa + (uintptr_t)a->bytes) continue;
-            const int64_t period = std::gcd(std::gcd(a->pitch0, a->pitch1),
-                                            std::gcd(b->pitch0, b->pitch1));
-            if (period > 0) {
-                int64_t off = (int64_t)(pb - pa) % period;
-                if (off < 0) off += period;
-                if (off >= a->width && off + b->width <= period) continue;
-            }
+            if (!may_meet(*a, *b)) continue;
             const Region &w = a->written ? *a : *b, &o = a->written ? *b : *a;
             return sg::fail(SIMTGO_EALIAS, "channels: %s: %s and %s were given overlapping device "
                             "memory, and the kernel writes through %s", K, w.name, o.name, w.name);
@@ -473,7 +505,7 @@ int check_codes(const char* K, const char* name, const void* codes, const void* 
 Region matrix(const char* name, const void* p, int64_t rows, int64_t pitch, int32_t channels,
               int32_t type, bool written) {
     const int64_t e = elem_size(type), apart = rows > 1 ? pitch * e : 0;
-    return {name, p, channels * e, apart, 0, (rows - 1) * apart + channels * e, written};
+    return {name, p, channels * e, apart, 0, (rows - 1) * apart + channels * e, written, rows, 1};
 }
 int64_t n_scales(int64_t rows, int32_t channels, int32_t block) {
     return rows * ((channels + (int64_t)block - 1) / block);

@@ -1370,7 +1370,7 @@ Region batch(const char* K, const char* name, const void* p, const simtgo_group_
              int64_t sample, int64_t row, bool written, int* rc) {
     const int64_t e = elem_size(c.type);
     const int64_t ns = c.samples > 1 ? sample : 0, nr = c.positions > 1 ? row : 0;
-    Region r = {name, p, c.channels * e, nr * e, ns * e, 0, written};
+    Region r = {name, p, c.channels * e, nr * e, ns * e, 0, written, c.positions, c.samples};
     if (*rc || !p) return r;
     if (ns < 0 || nr < 0 || ns > kMaxElems || nr > kMaxElems ||
         (__int128)(c.samples - 1) * ns + (__int128)(c.positions - 1) * nr > kMaxElems) {
