@@ -116,7 +116,7 @@ def _batch(t, name):
         return st[0], st[1]
     if sh[2] == 1:
         return st[0], st[1]
-    if sh[1] > 1 and st[1] != sh[2] * st[2]:
+    if t.numel() and sh[1] > 1 and st[1] != sh[2] * st[2]:
         raise TypeError(f"channels: the height and width of {name} must lie as one axis of rows")
     return st[0], st[2]
 
@@ -133,8 +133,8 @@ def _rows(t, name):
         raise TypeError(f"channels: the channels of {name} must be adjacent (stride 1)")
     if len(sh) == 1:
         return sh[0]
-    if len(sh) == 2:
-        return st[0]
+    if len(sh) == 2 or not t.numel():
+        return st[-2]
     pitch = run = None
     for n, s in zip(reversed(sh[:-1]), reversed(st[:-1])):
         if n == 1:

@@ -120,3 +120,18 @@ def test_overlaps_against_every_element(lib):
             free += 1
             assert rc != _lib.EALIAS, (n, s, c, sample, row, off)
     assert free > 300 and clash > 300
+
+
+def test_layouts_without_elements(calls):
+    for shape in ((2, 0, 8), (0, 3, 8), (2, 3, 0), (2, 0, 4, 8), (2, 3, 0, 8), (2, 5, 0)):
+        x = torch.zeros(*shape)
+        ch._rows(x, "x")
+        ch.Gated(x, x)
+        ch.Pack8(ch.NewCheckpoint(x, 32), x)
+        if shape[-1]:
+            ch._batch(x, "x")
+            ch.GroupNorm(x, x, groups=2)
+    ch._rows(torch.zeros(3, 4, 5, 8)[:, :0, :2], "x")
+    ch._batch(torch.zeros(3, 4, 5, 8)[:, :0, :2], "x")
+    with pytest.raises(TypeError, match="one pitch"):
+        ch._rows(torch.zeros(4, 6, 8)[:, :4], "x")
