@@ -1371,7 +1371,7 @@ Region batch(const char* K, const char* name, const void* p, const simtgo_group_
     const int64_t e = elem_size(c.type);
     const int64_t ns = c.samples > 1 ? sample : 0, nr = c.positions > 1 ? row : 0;
     Region r = {name, p, c.channels * e, nr * e, ns * e, 0, written, c.positions, c.samples};
-    if (*rc || !p) return r;
+    if (*rc || !p || !c.samples || !c.positions) return r;
     if (ns < 0 || nr < 0 || ns > kMaxElems || nr > kMaxElems ||
         (__int128)(c.samples - 1) * ns + (__int128)(c.positions - 1) * nr > kMaxElems) {
         *rc = sg::fail(SIMTGO_EARG, "channels: %s: %s has pitches of %lld and %lld elements", K,

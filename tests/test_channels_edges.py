@@ -135,3 +135,9 @@ def test_layouts_without_elements(calls):
     ch._batch(torch.zeros(3, 4, 5, 8)[:, :0, :2], "x")
     with pytest.raises(TypeError, match="one pitch"):
         ch._rows(torch.zeros(4, 6, 8)[:, :4], "x")
+
+
+def test_buffers_without_elements_do_not_overlap(lib):
+    for y in (4 * MB, 4 * MB + 4):
+        rc = forward(lib, norm_cfg(s=0, y_sample=0, x_sample=0), y, 4 * MB)
+        assert rc not in (_lib.EALIAS, _lib.EARG)

@@ -154,3 +154,18 @@ def test_the_largest_number_restores_to_a_finite_one():
         step = kept.scales.repeat_interleave(block, 1)[:, :64].to(O.F64)
         assert_within("restored", back, x.to(O.F64), step * 0.50002)
         assert kept.codes[0, 3] == 127 and kept.codes[1, 40] == -127 and (kept.codes[2] == 127).all()
+
+
+def test_calls_without_elements_by_any_axis():
+    for shape in ((2, 0, 8), (0, 3, 8), (2, 0, 4, 8), (2, 3, 0, 8)):
+        x = torch.empty(*shape, device="cuda")
+        y, dx, k = torch.empty_like(x), torch.empty_like(x), ch.NewCheckpoint(x, 32)
+        mean, rstd = torch.ones(2, shape[0], 2, device="cuda")
+        dw, db = torch.ones(2, 8, device="cuda")
+        ch.GroupNorm(y, x, groups=2, mean=mean, rstd=rstd, ckpt=k)
+        ch.GroupNormBackward(dx, dw, db, y, x, mean, rstd, groups=2)
+        assert (mean == 0).all() and (dw == 0).all() and (db == 0).all()
+        ch.Pack8(k, x)
+        ch.Unpack8(y, k)
+        ch.Gated(y, x, dx, a_ckpt=k)
+        ch.GatedBackward(dx, None, y, x)
