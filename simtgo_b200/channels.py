@@ -168,7 +168,8 @@ def _act(act):
     return k
 
 
-# Configurations by their values alone; the library copies one before it returns.
+# Configurations by their values alone (numbers: a tensor would be known by its
+# identity); the library copies one before it returns.
 @functools.lru_cache(maxsize=256)
 def _norm_cfg(*v):
     c = _lib.GroupNormConfig(*v)
@@ -244,7 +245,7 @@ def GroupNorm(y, x, weight=None, bias=None, *, groups, eps=1e-5, act="none", thr
         codes, scales = _kept(ckpt, x, "ckpt")
         block = ckpt.block
     cfg = _norm_cfg(xs, xr, ys, yr, 0, 0, n, s, c, groups, _type(x, "x"), pt, _act(act), block,
-                    threshold, eps)[1]
+                    float(threshold), float(eps))[1]
     _call("simtgo_GroupNorm", dev, stream, y.data_ptr(), mu, rs, x.data_ptr(), w, b, ln, codes,
           scales, cfg)
 
@@ -274,7 +275,7 @@ def GroupNormBackward(dx, dweight, dbias, dy, x, mean, rstd, weight=None, bias=N
         ds, dr = _batch(dx, "dx")
         dp = dx.data_ptr()
     cfg = _norm_cfg(xs, xr, ys, yr, ds, dr, n, s, c, groups, _type(dy, "dy"), pt, _act(act), block,
-                    threshold, eps)[1]
+                    float(threshold), float(eps))[1]
     _call("simtgo_GroupNorm_backward", dev, stream, dp,
           _flat(dweight, dy, c, torch.float32, "dweight"),
           _flat(dbias, dy, c, torch.float32, "dbias"), dy.data_ptr(), xp, codes, scales, mu, rs,
@@ -326,7 +327,8 @@ def Gated(y, a, b=None, *, act="silu", threshold=1.0, a_ckpt=None, b_ckpt=None, 
         bc, bsc = _kept(b_ckpt, a, "b_ckpt")
         block = b_ckpt.block
     rows, c = _matrix(a)
-    cfg = _gated_cfg(rows, ap, bp, yp, 0, 0, c, _type(a, "a"), _act(act), block, threshold, 0)[1]
+    cfg = _gated_cfg(rows, ap, bp, yp, 0, 0, c, _type(a, "a"), _act(act), block,
+                     float(threshold), 0)[1]
     _call("simtgo_Gated", dev, stream, y.data_ptr(), a.data_ptr(), bd, ac, asc, bc, bsc, cfg)
 
 
@@ -360,7 +362,7 @@ def GatedBackward(da, db, dy, a, b=None, *, act="silu", threshold=1.0, stream=No
     (ad, ac, asc, ap), (bd, bc, bsc, bp) = src
     rows, c = _matrix(dy)
     cfg = _gated_cfg(rows, ap, bp, yp, out[0][1], out[1][1], c, _type(dy, "dy"), _act(act), block,
-                     threshold, 0)[1]
+                     float(threshold), 0)[1]
     _call("simtgo_Gated_backward", dev, stream, out[0][0], out[1][0], dy.data_ptr(), ad, bd, ac,
           asc, bc, bsc, cfg)
 

@@ -141,3 +141,23 @@ def test_buffers_without_elements_do_not_overlap(lib):
     for y in (4 * MB, 4 * MB + 4):
         rc = forward(lib, norm_cfg(s=0, y_sample=0, x_sample=0), y, 4 * MB)
         assert rc not in (_lib.EALIAS, _lib.EARG)
+
+
+def test_options_are_read_at_every_call(calls):
+    """A number that the caller changes in place is another number."""
+    x = torch.zeros(2, 3, 8)
+    threshold, eps = torch.tensor(0.5), torch.tensor(1e-3)
+    m = torch.zeros(2, 2)
+    seen = []
+    for t, e in ((0.5, 1e-3), (0.75, 1e-2)):
+        threshold.fill_(t)
+        eps.fill_(e)
+        ch.GroupNorm(x, x, groups=2, act="softclip", threshold=threshold, eps=eps)
+        ch.GroupNormBackward(x, None, None, x, x, m, m, groups=2, act="softclip",
+                             threshold=threshold, eps=eps)
+        ch.Gated(x, x, act="softclip", threshold=threshold)
+        ch.GatedBackward(x, None, x, x, act="softclip", threshold=threshold)
+        got, calls[:] = [c[-1]._obj for c in calls], []
+        assert [round(c.act_param, 6) for c in got] == [t] * 4
+        seen.append([round(c.eps, 6) for c in got[:2]])
+    assert seen == [[1e-3] * 2, [1e-2] * 2]
