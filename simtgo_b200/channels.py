@@ -17,7 +17,8 @@ width, channels] (a channels_last NCHW tensor after permute(0, 2, 3, 1)), rows
 are any tensor whose last axis is the channels; the last axis has stride 1,
 the others any strides that need no copy. Element types are float32, bfloat16
 and float16. Calls are queued on `stream`, or on torch's current stream of the
-tensors' device, and not waited for. Nothing here records an autograd graph.
+tensors' device, and not waited for; a tensor may be freed after the call on
+either. Nothing here records an autograd graph.
 
 No counterpart in the reference; they stand beside Softclip, Quantize and
 WarpReduceSum (kernels/softclip.go:11, quantize.go:16, warpreduce.go:21).
@@ -189,10 +190,15 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _call(name, dev, stream, *args):
+def _call(name, dev, stream, tensors, *args):
     """Runs the library's function on device dev, on the caller's stream or on
-    torch's current one."""
-    sp = _raw_stream(dev) if stream is None else getattr(stream, "cuda_stream", stream)
+    torch's current one. On another stream than the current one the tensors'
+    memory is kept from new tensors until the call is done there."""
+    if stream is None:
+        sp = _raw_stream(dev)
+    else:
+        sp = getattr(stream, "cuda_stream", stream)
+        sp = getattr(sp, "value", sp) or 0   # a ctypes pointer
     fn = getattr(_lib._lib or _lib.load(), name)
     if dev == _device():
         rc = fn(*args, sp)
@@ -201,6 +207,13 @@ def _call(name, dev, stream, *args):
             rc = fn(*args, sp)
     if rc:
         check(rc)
+    if stream is not None and sp != _raw_stream(dev):
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(sp, device=dev)
+        for t in tensors:
+            for v in (t.codes, t.scales) if isinstance(t, Checkpoint) else (t,):
+                if v is not None:
+                    v.record_stream(stream)
 
 
 def _on_gpu(t, name):
@@ -246,8 +259,8 @@ def GroupNorm(y, x, weight=None, bias=None, *, groups, eps=1e-5, act="none", thr
         block = ckpt.block
     cfg = _norm_cfg(xs, xr, ys, yr, 0, 0, n, s, c, groups, _type(x, "x"), pt, _act(act), block,
                     float(threshold), float(eps))[1]
-    _call("simtgo_GroupNorm", dev, stream, y.data_ptr(), mu, rs, x.data_ptr(), w, b, ln, codes,
-          scales, cfg)
+    _call("simtgo_GroupNorm", dev, stream, (y, x, weight, bias, mean, rstd, lengths, ckpt),
+          y.data_ptr(), mu, rs, x.data_ptr(), w, b, ln, codes, scales, cfg)
 
 
 def GroupNormBackward(dx, dweight, dbias, dy, x, mean, rstd, weight=None, bias=None, *, groups,
@@ -276,7 +289,8 @@ def GroupNormBackward(dx, dweight, dbias, dy, x, mean, rstd, weight=None, bias=N
         dp = dx.data_ptr()
     cfg = _norm_cfg(xs, xr, ys, yr, ds, dr, n, s, c, groups, _type(dy, "dy"), pt, _act(act), block,
                     float(threshold), float(eps))[1]
-    _call("simtgo_GroupNorm_backward", dev, stream, dp,
+    _call("simtgo_GroupNorm_backward", dev, stream,
+          (dx, dweight, dbias, dy, x, mean, rstd, weight, bias, lengths), dp,
           _flat(dweight, dy, c, torch.float32, "dweight"),
           _flat(dbias, dy, c, torch.float32, "dbias"), dy.data_ptr(), xp, codes, scales, mu, rs,
           w, b, ln, cfg)
@@ -290,8 +304,8 @@ def Pack8(ckpt, x, *, stream=None):
     pitch = _rows(x, "x")
     codes, scales = _kept(ckpt, x, "ckpt")
     rows, c = _matrix(x)
-    _call("simtgo_Pack8", dev, stream, codes, scales, x.data_ptr(), _type(x, "x"), rows, c,
-          pitch, ckpt.block)
+    _call("simtgo_Pack8", dev, stream, (ckpt, x), codes, scales, x.data_ptr(), _type(x, "x"), rows,
+          c, pitch, ckpt.block)
 
 
 def Unpack8(x, ckpt, *, stream=None):
@@ -300,8 +314,8 @@ def Unpack8(x, ckpt, *, stream=None):
     pitch = _rows(x, "x")
     codes, scales = _kept(ckpt, x, "ckpt")
     rows, c = _matrix(x)
-    _call("simtgo_Unpack8", dev, stream, x.data_ptr(), codes, scales, _type(x, "x"), rows, c,
-          pitch, ckpt.block)
+    _call("simtgo_Unpack8", dev, stream, (x, ckpt), x.data_ptr(), codes, scales, _type(x, "x"),
+          rows, c, pitch, ckpt.block)
 
 
 def Gated(y, a, b=None, *, act="silu", threshold=1.0, a_ckpt=None, b_ckpt=None, stream=None):
@@ -329,7 +343,8 @@ def Gated(y, a, b=None, *, act="silu", threshold=1.0, a_ckpt=None, b_ckpt=None, 
     rows, c = _matrix(a)
     cfg = _gated_cfg(rows, ap, bp, yp, 0, 0, c, _type(a, "a"), _act(act), block,
                      float(threshold), 0)[1]
-    _call("simtgo_Gated", dev, stream, y.data_ptr(), a.data_ptr(), bd, ac, asc, bc, bsc, cfg)
+    _call("simtgo_Gated", dev, stream, (y, a, b, a_ckpt, b_ckpt), y.data_ptr(), a.data_ptr(), bd,
+          ac, asc, bc, bsc, cfg)
 
 
 def GatedBackward(da, db, dy, a, b=None, *, act="silu", threshold=1.0, stream=None):
@@ -363,8 +378,8 @@ def GatedBackward(da, db, dy, a, b=None, *, act="silu", threshold=1.0, stream=No
     rows, c = _matrix(dy)
     cfg = _gated_cfg(rows, ap, bp, yp, out[0][1], out[1][1], c, _type(dy, "dy"), _act(act), block,
                      float(threshold), 0)[1]
-    _call("simtgo_Gated_backward", dev, stream, out[0][0], out[1][0], dy.data_ptr(), ad, bd, ac,
-          asc, bc, bsc, cfg)
+    _call("simtgo_Gated_backward", dev, stream, (da, db, dy, a, b), out[0][0], out[1][0],
+          dy.data_ptr(), ad, bd, ac, asc, bc, bsc, cfg)
 
 
 __all__ = ["Checkpoint", "NewCheckpoint", "GroupNorm", "GroupNormBackward", "Pack8", "Unpack8",

@@ -169,3 +169,23 @@ def test_calls_without_elements_by_any_axis():
         ch.Unpack8(y, k)
         ch.Gated(y, x, dx, a_ckpt=k)
         ch.GatedBackward(dx, None, y, x)
+
+
+def test_memory_freed_after_a_call_on_another_stream_waits_for_it():
+    """torch hands a freed tensor's memory to the next allocation unless it
+    knows of the stream that still reads it."""
+    side = torch.cuda.Stream()
+    for stream in (side, side.cuda_stream, C.c_void_p(side.cuda_stream)):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()   # no other memory of x's size is free
+        x = torch.full((1, 4096, 4096), 0.5, device="cuda")
+        y, kept = torch.empty_like(x), ch.NewCheckpoint(x)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)   # about a tenth of a second
+        at = x.data_ptr()
+        ch.GroupNorm(y, x, groups=32, ckpt=kept, stream=stream)
+        del x
+        other = torch.empty(1, 4096, 4096, device="cuda")
+        assert other.data_ptr() != at
+        torch.cuda.synchronize()
