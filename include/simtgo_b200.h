@@ -272,8 +272,8 @@ int simtgo_Histogram_allreduce_fused_overwrite(simtgo_comm* comm, int32_t* bins,
  * equal bits. Written buffers must not overlap any other buffer of the call,
  * nor a row another row of the same buffer (SIMTGO_EALIAS). Configurations are
  * HOST pointers, read before the call returns. Group norm takes stream-ordered
- * scratch from the library's pool where it needs any (captured, it belongs to
- * the graph): make the first call on a device before any stream capture. */
+ * scratch from the library's pool where it needs any; captured, it belongs to
+ * the graph, and a capture may hold the first call on a device. */
 
 /* Element types. */
 enum { SIMTGO_F32 = 0, SIMTGO_BF16 = 1, SIMTGO_F16 = 2 };

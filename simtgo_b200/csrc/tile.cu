@@ -861,20 +861,27 @@ int scratch_pool(cudaMemPool_t* out) {
     if (dev < 0 || dev >= 64) return sg::fail(SIMTGO_EDEVICE, "device %d out of range", dev);
     std::lock_guard<std::mutex> lk(g_pool_mu);
     if (!g_pool[dev]) {
+        // Makes nothing on a stream, but is refused to a thread that captures one
+        // unless the thread's mode is relaxed.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if ((rc = sg::cuda_status(cudaThreadExchangeStreamCaptureMode(&mode),
+                                  "cudaThreadExchangeStreamCaptureMode")))
+            return rc;
         cudaMemPoolProps props = {};
         props.allocType = cudaMemAllocationTypePinned;
         props.location.type = cudaMemLocationTypeDevice;
         props.location.id = dev;
         cudaMemPool_t pool;
-        if ((rc = sg::cuda_status(cudaMemPoolCreate(&pool, &props), "cudaMemPoolCreate")))
-            return rc;
-        uint64_t keep = 1ull << 30;
-        if ((rc = sg::cuda_status(
-                 cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep),
-                 "cudaMemPoolSetAttribute"))) {
-            cudaMemPoolDestroy(pool);
-            return rc;
+        rc = sg::cuda_status(cudaMemPoolCreate(&pool, &props), "cudaMemPoolCreate");
+        if (!rc) {
+            uint64_t keep = 1ull << 30;
+            rc = sg::cuda_status(
+                cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep),
+                "cudaMemPoolSetAttribute");
+            if (rc) cudaMemPoolDestroy(pool);
         }
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (rc) return rc;
         g_pool[dev] = pool;
     }
     *out = g_pool[dev];

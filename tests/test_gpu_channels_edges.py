@@ -189,3 +189,35 @@ def test_memory_freed_after_a_call_on_another_stream_waits_for_it():
         other = torch.empty(1, 4096, 4096, device="cuda")
         assert other.data_ptr() != at
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("before", ["nothing", "norm", "pack"])
+def test_a_capture_after_calls_that_took_no_scratch(before):
+    """A graph may hold calls that need scratch whether or not an earlier call
+    of the process took any."""
+    fresh_process(f"""
+        import torch
+        from simtgo_b200 import channels as ch
+        g = torch.Generator(device="cuda").manual_seed(1)
+        small = torch.randn(1, 8, 8, device="cuda", generator=g)
+        if {before!r} == "norm":
+            ch.GroupNorm(torch.empty_like(small), small, groups=1)
+        elif {before!r} == "pack":
+            ch.Pack8(ch.NewCheckpoint(small), small)
+        x = torch.randn(1, 30000, 40, device="cuda", generator=g)
+        y, dx = torch.zeros_like(x), torch.zeros_like(x)
+        mean, rstd = torch.zeros(2, 1, 5, device="cuda")
+        dw, db = torch.zeros(2, 40, device="cuda")
+
+        def step():
+            ch.GroupNorm(y, x, groups=5, mean=mean, rstd=rstd)
+            ch.GroupNormBackward(dx, dw, db, x, x, mean, rstd, groups=5)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (y, dx, dw, db)]
+        step()
+        assert all(torch.equal(a, b) for a, b in zip(got, (y, dx, dw, db)))
+        """)
