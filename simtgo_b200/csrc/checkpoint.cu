@@ -12,9 +12,12 @@
 // Measured on one B200 (6462 GB/s copied): 16384x4096 bf16 in blocks of 128
 // packed in 31 us and restored in 30 us (6.5 TB/s both); an 8192x8192 bf16 gated
 // unit with both inputs kept 84 us forward and 80 us backward from the kept
-// codes (6.5 and 6.7 TB/s). Rows off 16-byte boundaries cost more: their units are
-// moved by words or single elements, codes by bytes (8192x1111 bf16 packed and
-// restored in 46 us, 1.2 TB/s): the access instructions bound them.
+// codes (6.5 and 6.7 TB/s). Rows that cannot be walked flat cost more, for two reasons.
+// A tile is a whole number of rows' units, so that from 129 to 255 units the rest
+// of 256 threads idle (8192x1112 bf16, 139 units, packed in 11 us; 8192x2048 in
+// 10). And rows off 16-byte boundaries are moved by words or single elements,
+// codes by bytes (8192x1111 packed in 15 us and restored in 26, 1112 in 11 and 7,
+// all from L2).
 #include <algorithm>
 #include <cmath>
 #include <numeric>

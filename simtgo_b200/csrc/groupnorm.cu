@@ -20,17 +20,17 @@
 //   shared memory (what does not fit is read again, last rows first, from L2);
 //   the blocks exchange their sums over distributed shared memory, and each
 //   finishes its own rows. One launch, nothing in HBM between. 8x4096x320 bf16
-//   (82 KB a block, 256 blocks): 20 us with SiLU, of which 6 sum, 7 finish and 4
+//   (82 KB a block, 256 blocks): 21 us with SiLU, of which 7 sum, 7 finish and 4
 //   join and exchange; the HBM floor is 6.5. Backward 31 us, floor 9.7.
 // - k_stats, k_join, k_apply (and their backward forms): where too few such
 //   clusters exist to fill the GPU -- a few samples of very many positions --
 //   every SM takes a chunk of a sample's rows, the chunks' sums are joined by a
 //   small kernel, and a third pass walks the chunks from their ends, whose rows
-//   L2 still holds. One 518400x128 bf16 sample: 26 us for the sums (5.1 TB/s),
-//   90 us with the join and the GELU pass; the floor is 41. The last pass is
-//   bound by its arithmetic: exponential and reciprocal for every value, 55 % of
-//   the special-function unit and 60 % of the issue slots at 16 warps an SM. A
-//   4x16384x512 step, forward with its checkpoint and backward from it: 130 us.
+//   L2 still holds. One 518400x128 bf16 sample: 29 us for the sums (4.6 TB/s,
+//   profiled), 92 us with the join and the GELU pass; the floor is 41. The last
+//   pass is bound by its arithmetic: exponential and reciprocal for every value, 55 % of
+//   the special-function unit and 61 % of the issue slots at 16 warps an SM. A
+//   4x16384x512 step, forward with its checkpoint and backward from it: 129 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -44,9 +44,9 @@ using namespace chan;
 namespace {
 
 constexpr int kThreads = 256;
-// Blocks that an SM's registers hold, at least: three and four measured slower
-// (the 518400x128 sample 93 and 104 us, 90 with two), since shorter chunks pay
-// the sums' and joins' fixed costs more often.
+// Blocks that an SM's registers hold, at least, and chunks that an SM takes: three
+// and four of both measured slower (the 518400x128 sample 93 and 104 us, 90 with
+// two). Fewer registers and shorter chunks were not measured apart.
 constexpr int kBlocks = 2;
 constexpr int kAhead = 2;  // batches of a ring where rows do not stay; four measured the same
 constexpr int64_t kMaxElems = int64_t(1) << 46;
@@ -1517,7 +1517,7 @@ Plan make_plan(Batch& B, const simtgo_group_norm& c, const sg::DevInfo& d, bool 
         // the GPU, through 1600 GB/s, after about 5 us more of launches and joins.
         // Clusters that fill it reach the same rate, and keep a call up to 8 GB.
         // Measured both ways (us, clusters and chunks): 8x4096x320 bf16 forward
-        // 20 and 26, backward 31 and 34; 4x16384x512 bf16 forward with its
+        // 21 and 26, backward 31 and 34; 4x16384x512 bf16 forward with its
         // checkpoint 150 and 57, backward 81 and 75; 600x1000x96 bf16 forward 86
         // and 104, backward 180 and 151; 64x4096x1024 float32 forward 989 and 851;
         // above the limit 256x16384x1024 bf16 forward 4791 and 4364, backward 8295
